@@ -155,8 +155,9 @@ def _norm32(x):
 
 
 def _quantize32(x):
-    s = x.abs().amax(1).float() / 127
-    # the quotient in 64 bits: whether it rounds up or down is decided next to a border
+    # the scale is a / 127 rounded once (a division by a number becomes a product with its reciprocal on the GPU: in 64 bits
+    # that ends in the same 32), and the quotient is taken in 64 bits: it is rounded up or down next to a border
+    s = (x.abs().amax(1).double() / 127).float()
     return torch.round(x.double() / s.double()[:, None]).float(), s
 
 
