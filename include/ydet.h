@@ -456,6 +456,97 @@ int ydet_preprocess_u8(const ydet_u8_image* images /* device, N entries */, cons
                        void* out, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Operators over the channels of every pixel.  A map of N images, H x W pixels and C channels is `rows` = N*H*W rows; row r
+ * of a slice (base, ld, coff) starts at value r*ld + coff.  No counterpart among the reference's detectors, which normalise
+ * over batches only; its transformer blocks normalise over channels (yolov5_official/modules.py:331-597).
+ * ------------------------------------------------------------------------------------------ */
+/* Layer normalisation: y = (x - mean) * rstd * gamma + beta with the mean and variance of each row's C values,
+ * rstd = 1 / sqrt(var + eps).  gamma / beta: C values of param_dtype, or NULL (1 / 0).  mean, rstd (rows values each, fp32,
+ * both or neither): what the backward pass needs.  y has x's dtype; y may be x.  C <= 8192, rows < 2^31; any ld,
+ * and slices at any value's address (a row's result does not depend on where it lies). */
+typedef struct {
+    const void* x;
+    void* y;
+    const void* gamma;
+    const void* beta;
+    float* mean;
+    float* rstd;
+    int64_t rows;
+    int32_t C;
+    int32_t x_ld, x_coff, y_ld, y_coff;
+    int32_t dtype, param_dtype;
+    float eps;
+} ydet_layer_norm_desc;
+int ydet_layer_norm(const ydet_layer_norm_desc* d, void* stream);
+
+/* Its gradient, from the output's gradient dy, the input x and the statistics the forward pass left: dx (dtype, may be NULL),
+ * dgamma and dbeta (C values of param_dtype, each may be NULL).  dgamma and dbeta are sums over all rows in fp32, taken in a
+ * fixed order (the same bits every time); they need ydet_layer_norm_backward_workspace_bytes(rows, C) bytes of workspace.
+ * rows = 0 writes zeros to them.  dx may be dy. */
+typedef struct {
+    const void* dy;
+    const void* x;
+    void* dx;
+    const void* gamma;
+    const float* mean;
+    const float* rstd;
+    void* dgamma;
+    void* dbeta;
+    int64_t rows;
+    int32_t C;
+    int32_t dy_ld, dy_coff, x_ld, x_coff, dx_ld, dx_coff;
+    int32_t dtype, param_dtype;
+} ydet_layer_norm_grad_desc;
+size_t ydet_layer_norm_backward_workspace_bytes(int64_t rows, int C);
+int ydet_layer_norm_backward(const ydet_layer_norm_grad_desc* d, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rows in 8 bits, symmetric, one scale a row: scale = max|v| / 127 (rounded once to fp32), q = the integer nearest v / scale,
+ * ties to even (exactly: no rounding before that one), so |q| <= 127.  v is the row of x or, with normalize != 0, its layer
+ * normalisation (gamma, beta, eps as above) unrounded.  A row whose largest magnitude is below 127 * 2^-126 has scale 0 and
+ * q = 0; a row with a NaN or an infinity has scale NaN and q = 0, which makes every product with it NaN.
+ * q: rows of q_ld bytes (a multiple of 16, at least C), 16-byte aligned; bytes C up to the next multiple of 16 are written as
+ * zero.  C <= 8192. */
+typedef struct {
+    const void* x;
+    int8_t* q;
+    float* scale;
+    const void* gamma;
+    const void* beta;
+    int64_t rows;
+    int32_t C;
+    int32_t x_ld, x_coff, q_ld;
+    int32_t dtype, param_dtype;
+    int32_t normalize;
+    float eps;
+} ydet_quantize_desc;
+int ydet_quantize_rows_i8(const ydet_quantize_desc* d, void* stream);
+
+/* Product in 8-bit integers -- a 1x1 convolution over rows that ydet_quantize_rows_i8 wrote:
+ *   acc[r, n] = sum_k x[r, k] * w[n, k]      (exact 32-bit integers; K <= 131071)
+ *   y[r, n]   = act(acc * x_scale[r] * w_scale[n] + bias[n])  with the residual as in ydet_conv2d_nhwc (res_mode; res has y's dtype)
+ * w [n_pad][kp], rows >= N and columns >= K zero, n_pad a multiple of 128, kp a multiple of 64; w_scale and bias (may be NULL)
+ * hold n_pad values; all three 16-byte aligned.  x may lie anywhere; slices that are 16-byte aligned with x_ld a multiple
+ * of 16 are read in 16-byte pieces (the bytes behind K in a row's last piece are read, their values do not matter; the
+ * slice's row has to hold them).  y may be res.  x_ld <= 2^23, rows < 2^31 - 512. */
+typedef struct {
+    const int8_t* x;
+    const float* x_scale;
+    const int8_t* w;
+    const float* w_scale;
+    const float* bias;
+    const void* res;
+    void* y;
+    int64_t rows;
+    int32_t K, N, kp, n_pad;
+    int32_t x_ld, x_coff, y_ld, y_coff, res_ld, res_coff;
+    int32_t act;      /* ydet_act */
+    float slope;
+    int32_t res_mode; /* ydet_res_mode */
+    int32_t out_dtype;/* dtype of y and res */
+} ydet_matmul_i8_desc;
+int ydet_matmul_i8(const ydet_matmul_i8_desc* d, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Launch-list executor: one call runs a whole pre-planned forward pass
  * (the Python loop of Model.forward_once, yolov5_official/model.py:220-234, and the forward()
  * bodies of models/v2d19.py, v3tiny.py, v3spp.py, v4.py).

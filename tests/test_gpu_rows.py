@@ -1,0 +1,514 @@
+"""Layer normalisation, row quantisation and the 8-bit product (yolo_amd.ops) against plain 64-bit implementations.
+
+Tolerances are bounds on the rounding errors, written out where they are used: u = 2^-24 is half a step of fp32, half(t) half
+a step of the stored type relative to the value.  A row's fp32 sum goes through at most 32 values one after the other in a lane and
+a tree of 8 levels: its error is at most 40 u times the sum of magnitudes.
+"""
+import math
+
+import pytest
+import torch
+
+from yolo_amd import _ffi, ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0 ** -24
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def half(t):
+    return torch.finfo(t).eps / 2
+
+
+def gen(seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    return g
+
+
+def randn(g, *shape, dtype=F32):
+    return torch.randn(*shape, generator=g, device=DEV).to(dtype)
+
+
+def within(got, want, bound):
+    """|got - want| <= bound everywhere; infinities and NaN in the same places."""
+    got, want = got.double(), want.double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    fine = torch.isfinite(want)
+    assert torch.equal(got[~fine & ~torch.isnan(want)], want[~fine & ~torch.isnan(want)])
+    over = (got - want).abs()[fine] - bound.expand_as(want)[fine]
+    assert over.numel() == 0 or over.max() <= 0, f"off by {over.max():.3g} over the bound at most"
+
+
+# ---- plain implementations in 64 bits --------------------------------------------------------------------------------------
+def norm64(x, w, b, eps):
+    x = x.double()
+    mean = x.mean(-1, keepdim=True)
+    rstd = 1 / torch.sqrt(((x - mean) ** 2).mean(-1, keepdim=True) + eps)
+    xh = (x - mean) * rstd
+    y = xh
+    if w is not None:
+        y = y * w.double()
+    if b is not None:
+        y = y + b.double()
+    return y, xh, rstd
+
+
+def xh_error(x, xh, rstd):
+    """Bound on the error of (x - mean) * rstd in fp32: the mean is off by at most 41 u mean|x|, the variance by 44 u of itself
+    (a shift of the mean moves it in second order only), rstd by 25 u, two more roundings."""
+    return 64 * U * (x.double().abs().mean(-1, keepdim=True) * rstd + xh.abs())
+
+
+def quant64(v):
+    """(q, scale) of rows in 64 bits, from the definition."""
+    v = v.double()
+    top = v.abs().amax(-1)
+    bad = ~torch.isfinite(v).all(-1)
+    top = torch.where(bad, 0.0, top.nan_to_num(0.0, 0.0, 0.0))
+    some = top >= float(torch.tensor(127.0) * torch.tensor(1.17549435e-38))
+    s = torch.where(some, (top / 127).float().double(), 1.0)
+    q = torch.round(torch.where(some[..., None], v, 0.0) / s[..., None])
+    scale = torch.where(some, s, 0.0)
+    scale[bad] = float("nan")
+    return q.to(torch.int8), scale.float()
+
+
+def product64(q, s, wq, ws, bias, act, slope, res, mode):
+    """(y, bound without the stored type's half step)."""
+    acc = q.double() @ wq.double().t().contiguous()          # exact: integers below 2^53
+    p = acc * s.double()[..., None] * ws.double()
+    b = bias.double() if bias is not None else torch.zeros_like(ws).double()
+    v = p + b
+    e = 5 * U * (p.abs() + b.abs())               # the sum's conversion, two products, the sum with the bias
+    if res is not None and mode == "before":
+        v = v + res.double()
+        e = e + U * (v.abs() + p.abs() + b.abs())
+    if act == "silu":
+        # exp2 and reciprocal of the hardware are one step (2 u) off each, exp2's argument two roundings of |v| log2(e)
+        y = v * torch.sigmoid(v)
+        e = 1.1 * e + (3 * v.abs() + 8) * U * y.abs()
+    elif act == "leaky":
+        y = torch.where(v > 0, v, v * float(torch.tensor(slope, dtype=F32)))
+        e = e * max(1.0, abs(slope)) + U * y.abs()
+    else:
+        y = v
+    if res is not None and mode == "after":
+        e = e + U * (y.abs() + res.double().abs())
+        y = y + res.double()
+    return y, e
+
+
+# ---- layer norm ----------------------------------------------------------------------------------------------------------
+SIZES = [(1, 1), (1, 16), (3, 7), (5, 8), (64, 24), (257, 32), (1, 75), (33, 64), (129, 128), (17, 255), (400, 512), (65, 513), (9, 1000),
+         (31, 1024), (12, 2048), (7, 2050), (3, 4096), (2, 5001), (2, 8192)]
+
+
+@pytest.mark.parametrize("dtype,pdtype", [(F32, F32), (BF16, F32), (BF16, BF16), (F32, BF16)])
+@pytest.mark.parametrize("rows,C", SIZES)
+def test_layer_norm_forward_and_backward(rows, C, dtype, pdtype):
+    g = gen(rows * 10007 + C)
+    x = (randn(g, rows, C) * (0.2 + randn(g, C).abs()) + randn(g, C)).to(dtype)
+    w, b = (1 + 0.3 * randn(g, C)).to(pdtype), (0.3 * randn(g, C)).to(pdtype)
+    dy = randn(g, rows, C, dtype=dtype)
+    eps = 1e-5
+    y64, xh, rstd = norm64(x, w, b, eps)
+    ex = xh_error(x, xh, rstd)
+    y, mean, rs = ops.layer_norm_forward(x, w, b, eps)
+    assert y.dtype == dtype and mean.shape == rs.shape == (rows,)
+    # y = xh w + b: one fused rounding on top of xh's error, then the stored type's
+    within(y, y64, ex * w.double().abs() + 2 * U * ((xh * w.double()).abs() + b.double().abs()) + half(dtype) * y64.abs() * (1 + 1e-6) + 1e-30)
+    assert torch.equal(y, ops.layer_norm(x, w, b, eps))
+
+    dx, dw, db = ops.layer_norm_backward(dy, x, mean, rs, w)
+    assert dx.dtype == dtype and dw.dtype == db.dtype == pdtype
+    d = dy.double()
+    t = d * w.double()
+    m1, m2 = t.mean(-1, keepdim=True), (t * xh).mean(-1, keepdim=True)
+    dx64 = rstd * (t - m1 - xh * m2)
+    # g = dy w rounds once; each of the row's two sums is off by 44 u of its magnitudes and by the error of xh under it; the
+    # final expression has four roundings of its terms; rstd's own 25 u multiply the whole
+    e = rstd * (64 * U * (t.abs() + t.abs().mean(-1, keepdim=True) + xh.abs() * (t * xh).abs().mean(-1, keepdim=True))
+                + xh.abs() * (t.abs() * ex).mean(-1, keepdim=True) + ex * m2.abs())
+    e = e + 32 * U * rstd * (t.abs() + m1.abs() + (xh * m2).abs())
+    within(dx, dx64, e + half(dtype) * (dx64.abs() + e))
+    # sums over rows: at most 200 values one after the other in a lane group and 150 behind that (groups of a workgroup, workgroups)
+    n = min(rows, 200) + 150
+    dw64, db64 = (d * xh).sum(0), d.sum(0)
+    ew = n * U * (d * xh).abs().sum(0) + (d.abs() * ex).sum(0)
+    within(dw, dw64, ew + half(pdtype) * (dw64.abs() + ew))
+    eb = n * U * d.abs().sum(0)
+    within(db, db64, eb + half(pdtype) * (db64.abs() + eb))
+
+
+@pytest.mark.parametrize("rows,C,dtype", [(100000, 32, BF16), (40000, 128, F32), (70001, 33, BF16), (20000, 512, BF16), (9000, 2048, F32)])
+def test_layer_norm_many_rows(rows, C, dtype):
+    """Sizes at which every lane group takes several rows and the workspace all its workgroups."""
+    g = gen(C)
+    x, dy = randn(g, rows, C, dtype=dtype) + 0.5, randn(g, rows, C, dtype=dtype)
+    w, b = 1 + 0.3 * randn(g, C), 0.3 * randn(g, C)
+    y64, xh, rstd = norm64(x, w, b, 1e-5)
+    ex = xh_error(x, xh, rstd)
+    y, mean, rs = ops.layer_norm_forward(x, w, b)
+    within(y, y64, ex * w.double().abs() + 2 * U * ((xh * w.double()).abs() + b.double().abs()) + half(dtype) * y64.abs() * (1 + 1e-6) + 1e-30)
+    dx, dw, db = ops.layer_norm_backward(dy, x, mean, rs, w)
+    d = dy.double()
+    # rows of one lane group: at most 1024 workgroups of at least 4 groups, but no fewer than 8 rows each
+    n = max(8, math.ceil(rows / 1024)) + 200
+    ew = n * U * (d * xh).abs().sum(0) + (d.abs() * ex).sum(0)
+    within(dw, (d * xh).sum(0), ew + half(F32) * ew + U * (d * xh).sum(0).abs())
+    within(db, d.sum(0), n * U * d.abs().sum(0) + U * d.sum(0).abs())
+    again = ops.layer_norm_backward(dy, x, mean, rs, w)
+    assert all(torch.equal(p, q) for p, q in zip((dx, dw, db), again)), "the same call gives other bits"
+
+
+def test_layer_norm_gradient_against_differences():
+    """dx, dw, db along random directions against central differences of the 64-bit forward pass; the differences' own error is
+    what halving the step changes."""
+    g = gen(5)
+    x, w, b, dy = randn(g, 6, 37), 1 + 0.3 * randn(g, 37), randn(g, 37), randn(g, 6, 37)
+    xl, wl, bl = (t.clone().requires_grad_(True) for t in (x, w, b))
+    got = torch.autograd.grad(ops.layer_norm(xl, wl, bl), (xl, wl, bl), dy)
+    loss = lambda a: (norm64(a[0], a[1], a[2], 1e-5)[0] * dy.double()).sum()
+    for k in range(3):
+        base = [x.double(), w.double(), b.double()]
+        v = randn(g, *base[k].shape).double()
+
+        def slope(h):
+            up, dn = list(base), list(base)
+            up[k], dn[k] = base[k] + h * v, base[k] - h * v
+            return float((loss(up) - loss(dn)) / (2 * h))
+        d1, d2 = slope(1e-4), slope(5e-5)
+        # the gradient's fp32 entries are off by about 100 u of their terms' magnitude (the bounds of the test above)
+        tol = 2 * abs(d1 - d2) + 200 * U * float((got[k].double().abs() + 1).mul(v.abs()).sum()) + 1e-9
+        assert abs(float((got[k].double() * v).sum()) - d2) <= tol, (k, d1, d2)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_layer_norm_autograd_partial_and_broadcast(dtype):
+    g = gen(8)
+    x, dy = randn(g, 2, 5, 3, 48, dtype=dtype), randn(g, 2, 5, 3, 48, dtype=dtype)
+    w, b = (1 + 0.2 * randn(g, 48)), randn(g, 48, dtype=BF16)
+    y, mean, rs = ops.layer_norm_forward(x, w, b)
+    full = ops.layer_norm_backward(dy, x, mean, rs, w)
+    for need in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 0, 1), (1, 1, 1)):
+        xs = x.clone().requires_grad_(bool(need[0]))
+        ws, bs = w.clone().requires_grad_(bool(need[1])), b.clone().requires_grad_(bool(need[2]))
+        out = ops.layer_norm(xs, ws, bs)
+        assert torch.equal(out.detach(), y)
+        out.backward(dy)
+        for k, (t, f) in enumerate(zip((xs, ws, bs), full)):
+            if need[k]:
+                assert t.grad.dtype == t.dtype and torch.equal(t.grad, f.to(t.dtype))
+            else:
+                assert t.grad is None
+    # no weight, no bias; a broadcast input and a broadcast output gradient
+    one = x[:, :1, :1].clone().requires_grad_(True)
+    z = ops.layer_norm(one.expand(2, 5, 3, 48))
+    z.sum().backward()
+    zz, mm, rr = ops.layer_norm_forward(one.detach().expand(2, 5, 3, 48).contiguous())
+    assert torch.equal(z.detach(), zz)
+    dx = ops.layer_norm_backward(torch.ones_like(zz), one.detach().expand(2, 5, 3, 48).contiguous(), mm, rr)[0]
+    assert torch.equal(one.grad, dx.sum((1, 2), keepdim=True))
+    # weight used twice: its gradient is the sum of both
+    ws = w.clone().requires_grad_(True)
+    (ops.layer_norm(x, ws).float().sum() + ops.layer_norm(x, ws).float().sum()).backward()
+    ones = ops.layer_norm_backward(torch.ones_like(y), x, mean, rs, w)[1]
+    assert torch.equal(ws.grad, ones + ones)
+
+
+def test_layer_norm_special_rows():
+    """Infinities and NaN stay in their rows; constant and empty rows; a row far from zero."""
+    g = gen(3)
+    x = randn(g, 7, 40)
+    x[1, 3], x[2, 5], x[4] = float("nan"), float("inf"), 2.5
+    x[5] += 1000.0
+    y = ops.layer_norm(x)
+    assert torch.isnan(y[1]).all() and torch.isnan(y[2]).all()
+    assert torch.equal(y[4], torch.zeros(40, device=DEV))
+    y64, xh, rstd = norm64(x[[0, 3, 5, 6]], None, None, 1e-5)
+    within(y[[0, 3, 5, 6]], y64, xh_error(x[[0, 3, 5, 6]], xh, rstd) + 4 * U * y64.abs())
+    for shape in ((0, 40), (2, 0, 40)):
+        e = torch.empty(shape, device=DEV)
+        out, m, r = ops.layer_norm_forward(e)
+        assert out.shape == shape and m.shape == shape[:-1]
+        w = torch.ones(40, device=DEV, requires_grad=True)
+        b = torch.ones(40, device=DEV, requires_grad=True)
+        ops.layer_norm(e, w, b).sum().backward()
+        assert torch.equal(w.grad, torch.zeros(40, device=DEV)) and torch.equal(b.grad, torch.zeros(40, device=DEV))
+        q, s = ops.quantize_rows(e)
+        assert q.shape == shape and s.shape == shape[:-1]
+
+
+# ---- rows in 8 bits -------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,C", SIZES)
+def test_quantize_rows(rows, C, dtype):
+    """Equal, value by value, to the definition in 64 bits; zeros up to the row's 16-byte border."""
+    g = gen(rows * 31 + C)
+    x = (randn(g, rows, C) * torch.exp(3 * randn(g, rows, 1))).to(dtype)
+    q, s = ops.quantize_rows(x)
+    q64, s64 = quant64(x)
+    assert torch.equal(s, s64) and torch.equal(q, q64)
+    if q.stride(0) != C and rows:
+        full = q.as_strided((rows, q.stride(0)), (q.stride(0), 1))
+        assert full.shape[1] % 16 == 0 and not full[:, C:].any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_quantize_rows_borders_and_special_rows(dtype):
+    """Values on and next to the borders between two steps, rows of zeros, the smallest and the largest numbers, NaN, infinity."""
+    k = torch.arange(-127, 127, device=DEV).double() + 0.5
+    rows = [torch.cat([k, k.new_tensor([127.0, -127.0])])]                      # scale 1: every value a tie
+    for s in (0.37, 3.0, 1e-30, 1e30, 2.0 ** -126):
+        near = torch.cat([k * s, k.new_tensor([127.0 * s, -127.0 * s])])
+        rows += [near, near * (1 + 1e-7), near * (1 - 1e-7), near.roll(1) / 3]
+    fm = torch.finfo(dtype)
+    rows += [torch.zeros(256, device=DEV).double(), torch.full((256,), fm.max, device=DEV).double(),
+             torch.full((256,), fm.smallest_normal, device=DEV).double(), torch.full((256,), fm.smallest_normal / 4, device=DEV).double(),
+             k.new_tensor([1.49e-36] * 256), k.new_tensor([1.51e-36] * 256)]
+    x = torch.stack(rows).to(dtype)
+    bad = x[:4].clone()
+    bad[0, 0], bad[1, 77], bad[2, 255], bad[3, 3] = float("nan"), float("inf"), float("-inf"), float("nan")
+    x = torch.cat([x, bad, x[:3]])
+    q, s = ops.quantize_rows(x)
+    q64, s64 = quant64(x)
+    assert torch.equal(s.nan_to_num(-1), s64.nan_to_num(-1)) and torch.equal(q, q64)
+    assert torch.isnan(s[-7:-3]).all() and not q[-7:-3].any()
+    y = ops.matmul_i8(q, s, ops.LinearI8.quantize(torch.randn(5, 256, device=DEV)))
+    assert torch.isnan(y[-7:-3]).all() and torch.isfinite(y[:1]).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,C", [(1, 1), (3, 7), (64, 24), (17, 255), (400, 512), (31, 1024), (7, 2050), (2, 8192), (30000, 64)])
+def test_layer_norm_quantize(rows, C, dtype):
+    """The steps of the fused form stand for the norm's values to half a step, and the scale is the row's largest value."""
+    g = gen(C * 7 + rows)
+    x = randn(g, rows, C, dtype=dtype) * 2 + 0.3
+    w, b = 1 + 0.3 * randn(g, C), 0.3 * randn(g, C)
+    q, s = ops.layer_norm_quantize(x, w, b)
+    y64, xh, rstd = norm64(x, w, b, 1e-5)
+    e = (xh_error(x, xh, rstd) * w.double().abs() + 2 * U * ((xh * w.double()).abs() + b.double().abs()))
+    top = y64.abs().amax(-1)
+    within(s, top / 127, (e.amax(-1) + 2 * U * top) / 127)
+    within(q.double() * s.double()[:, None], y64, e + 0.5 * s.double()[:, None] * (1 + 4 * U) + 127 * U * s.double()[:, None])
+
+
+# ---- product ------------------------------------------------------------------------------------------------------------------
+def operands(g, M, K, N, full=False):
+    q = torch.randint(-128 if full else -127, 128, (M, K), generator=g, device=DEV, dtype=torch.int8)
+    wq = torch.randint(-128 if full else -127, 128, (N, K), generator=g, device=DEV, dtype=torch.int8)
+    s, ws = torch.rand(M, generator=g, device=DEV) * 0.01, torch.rand(N, generator=g, device=DEV) * 0.01
+    return q, s, wq, ws, randn(g, N)
+
+
+PRODUCTS = [(1, 1, 1), (1, 64, 16), (2, 1024, 1024), (16, 100, 33), (17, 128, 128), (63, 65, 75), (100, 1000, 255), (128, 128, 128),
+            (129, 192, 144), (400, 1024, 512), (1000, 64, 48), (2888, 1000, 255), (4097, 256, 130), (9000, 320, 255), (20000, 48, 512),
+            (3000, 4096, 1024), (30001, 16, 24)]
+
+
+@pytest.mark.parametrize("out", [F32, BF16])
+@pytest.mark.parametrize("M,K,N", PRODUCTS)
+def test_matmul_i8(M, K, N, out):
+    g = gen(M + 3 * K + 7 * N)
+    q, s, wq, ws, bias = operands(g, M, K, N, full=True)
+    res = randn(g, M, N, dtype=out)
+    lin, bare = ops.LinearI8(wq, ws, bias), ops.LinearI8(wq, ws)
+    for act, mode, r, l in (("none", "after", None, bare), ("silu", "after", res, lin), ("leaky", "before", res, lin), ("silu", "before", None, lin)):
+        y = ops.matmul_i8(q, s, l, act=act, slope=0.1, res=r, res_mode=mode, out_dtype=out)
+        want, e = product64(q, s, wq, ws, bias if l is lin else None, act, 0.1, r, mode)
+        assert y.shape == (M, N) and y.dtype == out
+        within(y, want, e + half(out) * (want.abs() + e) + 1e-37)
+
+
+@pytest.mark.parametrize("K", [131071, 20000])
+def test_matmul_i8_longest_sums(K):
+    """The largest sums a 32-bit integer has to hold."""
+    q = torch.full((3, K), -128, device=DEV, dtype=torch.int8)
+    q[1] = 127
+    wq = torch.full((20, K), -128, device=DEV, dtype=torch.int8)
+    wq[7:] = 127
+    s, ws = torch.ones(3, device=DEV), torch.ones(20, device=DEV)
+    y = ops.matmul_i8(q, s, ops.LinearI8(wq, ws), out_dtype=F32)
+    want = q.cpu().double() @ wq.cpu().double().t()
+    assert torch.equal(y.cpu(), want.float())
+
+
+@pytest.mark.parametrize("out", [F32, BF16])
+def test_matmul_i8_does_not_depend_on_the_batch(out):
+    """Whichever kernel takes the rows: a row's result is the same alone, among few and among many."""
+    g = gen(77)
+    q, s, wq, ws, bias = operands(g, 40000, 512, 256)
+    lin = ops.LinearI8(wq, ws, bias)
+    y = ops.matmul_i8(q, s, lin, act="silu", out_dtype=out)
+    for n in (1, 16, 17, 300, 1000, 5000, 20000):
+        assert torch.equal(ops.matmul_i8(q[:n], s[:n], lin, act="silu", out_dtype=out), y[:n])
+
+
+def test_rows_at_any_distance_and_address():
+    """Channel slices of wider maps, odd pitches and addresses, transposed and broadcast maps."""
+    g = gen(21)
+    for dtype in (F32, BF16):
+        big = randn(g, 3, 10, 11, 70, dtype=dtype)
+        w, b = randn(g, 64), randn(g, 64)
+        for x in (big[..., :64], big[..., 1:65], big[..., 6:70], big[:, 1:9, 2:7, 3:67], big[..., :64].transpose(0, 1), big[0, 0, 0, :64],
+                  big[:, :1, :, :64].expand(3, 10, 11, 64), big[:, :, :, :64][:, ::2]):
+            ref = x.contiguous().clone()
+            assert torch.equal(ops.layer_norm(x, w, b), ops.layer_norm(ref, w, b))
+            for a, c in zip(ops.quantize_rows(x) + ops.layer_norm_quantize(x, w, b), ops.quantize_rows(ref) + ops.layer_norm_quantize(ref, w, b)):
+                assert torch.equal(a, c)
+            y, m, r = ops.layer_norm_forward(ref, w, b)
+            dy = randn(g, *ref.shape, dtype=dtype)
+            wide = torch.zeros(*ref.shape[:-1], 71, device=DEV, dtype=dtype)
+            wide[..., 5:69] = dy
+            for a, c in zip(ops.layer_norm_backward(wide[..., 5:69], x, m, r, w), ops.layer_norm_backward(dy, ref, m, r, w)):
+                assert torch.equal(a, c)
+    # 8-bit rows: any pitch and address, the last row at the very end of its memory
+    q, s, wq, ws, bias = operands(g, 200, 77, 40)
+    lin = ops.LinearI8(wq, ws, bias)
+    want = ops.matmul_i8(q, s, lin)
+    for pitch, off in ((77, 0), (80, 0), (80, 3), (96, 16), (101, 5), (128, 32)):
+        flat = torch.randint(-127, 128, (199 * pitch + off + 77,), generator=g, device=DEV, dtype=torch.int8)
+        v = flat.as_strided((200, 77), (pitch, 1), off)
+        v.copy_(q)
+        assert torch.equal(ops.matmul_i8(v, s, lin), want), (pitch, off)
+    wide = torch.zeros(200, 60, device=DEV)
+    r = randn(g, 200, 40)
+    wide[:, 3:43] = r
+    assert torch.equal(ops.matmul_i8(q, s, lin, res=wide[:, 3:43], out_dtype=F32), ops.matmul_i8(q, s, lin, res=r, out_dtype=F32))
+
+
+def test_rows_beyond_32_bit_offsets():
+    """Maps whose last rows lie more than 2^32 bytes and 2^31 values behind the first."""
+    rows, ld = 70001, 40000
+    big = torch.empty(rows, ld, device=DEV, dtype=BF16)            # 5.6 GB, touched in a few columns
+    x = big[:, 64:128]
+    g = gen(1)
+    x.copy_(randn(g, rows, 64))
+    ref = x.contiguous()
+    assert torch.equal(ops.layer_norm(x), ops.layer_norm(ref))
+    q, s = ops.quantize_rows(x)
+    q2, s2 = ops.quantize_rows(ref)
+    assert torch.equal(q, q2) and torch.equal(s, s2)
+    lin = ops.LinearI8.quantize(randn(g, 48, 64))
+    want = ops.matmul_i8(q, s, lin)
+    wide8 = big.view(torch.int8)[:, 16:80]                         # 8-bit rows 80 000 bytes apart
+    wide8.copy_(q)
+    assert torch.equal(ops.matmul_i8(wide8, s, lin), want)
+    # the library's own slices: output rows that far apart
+    d = _ffi.MatmulI8Desc(q.data_ptr(), s.data_ptr(), lin.w.data_ptr(), lin.scale.data_ptr(), None, None, big.data_ptr(), rows, 64, 48,
+                          lin.kp, lin.n_pad, 64, 0, ld, 1024, 0, 0, 0, 0.0, 0, _ffi.BF16)
+    _ffi.check(_ffi.lib().ydet_matmul_i8(d, _ffi.current_stream()))
+    assert torch.equal(big[:, 1024:1072], want)
+
+
+def test_a_token_wise_block():
+    """norm -> 8 bits -> 256 channels, SiLU -> 8 bits -> 64 channels + shortcut, as a network runs it: every product within its
+    bound of the 64-bit one on the rows it was given, and the whole near the floating block."""
+    g = gen(12)
+    N, H, W, C = 2, 13, 13, 64
+    x = randn(g, N, H, W, C, dtype=BF16)
+    w, b = 1 + 0.2 * randn(g, C), 0.1 * randn(g, C)
+    w1, w2 = randn(g, 256, C) / 8, randn(g, C, 256) / 16
+    l1, l2 = ops.LinearI8.quantize(w1, randn(g, 256)), ops.LinearI8.quantize(w2[:, :, None, None])
+    q, s = ops.layer_norm_quantize(x, w, b)
+    h = ops.matmul_i8(q, s, l1, act="silu")
+    y = ops.linear_i8(h, l2, res=x)
+    assert h.shape == (N, H, W, 256) and y.shape == x.shape and y.dtype == BF16
+    want, e = product64(q, s, l1.w[:256, :C], l1.scale[:256], l1.bias[:256], "silu", 0.1, None, "after")
+    within(h, want, e + half(BF16) * (want.abs() + e))
+    q2, s2 = ops.quantize_rows(h)
+    want, e = product64(q2, s2, l2.w[:C, :256], l2.scale[:C], None, "none", 0.1, x, "after")
+    within(y, want, e + half(BF16) * (want.abs() + e))
+    # the floating block: 8 bits put noise of uniform half steps on rows and weights, amax / 127 / sqrt(12) each per value
+    z = norm64(x, w, b, 1e-5)[0]
+    hz = z @ w1.double().t() + l1.bias[:256].double()
+    hz = hz * torch.sigmoid(hz)
+    yz = hz @ w2.double().t() + x.double()
+    assert float((y.double() - yz).norm() / (yz - x.double()).norm()) < 0.05
+
+
+# ---- streams, graphs -------------------------------------------------------------------------------------------------------
+def test_streams_and_graph_replays():
+    """A block captured into a graph: every replay, with eager work and synchronisations between, equals the eager result; two
+    streams at once give what one gives."""
+    g = gen(14)
+    x, dy = randn(g, 4097, 96, dtype=BF16), randn(g, 4097, 96, dtype=BF16)
+    w, b = 1 + 0.2 * randn(g, 96), randn(g, 96)
+    lin = ops.LinearI8.quantize(randn(g, 128, 96))
+
+    def block(x, dy):
+        y, m, r = ops.layer_norm_forward(x, w, b)
+        grads = ops.layer_norm_backward(dy, x, m, r, w)
+        q, s = ops.layer_norm_quantize(x, w, b)
+        return (y,) + grads + (ops.matmul_i8(q, s, lin, act="silu"), ops.linear_i8(x[:7], lin), ops.linear_i8(x, lin, out_dtype=F32))
+    sx, sdy = x.clone(), dy.clone()
+    block(sx, sdy)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = block(sx, sdy)
+    second = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(second):
+        out2 = block(sx, sdy)
+    for k in range(4):
+        sx.copy_(x * (k + 1))
+        sdy.copy_(dy.roll(k, 0))
+        want = block(sx.clone(), sdy.clone())
+        graph.replay()
+        second.replay()
+        torch.cuda.synchronize()
+        for a, c, e in zip(out, want, out2):
+            assert torch.equal(a, c) and torch.equal(e, c)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    want = [block(x * k, dy) for k in (1, 2)]
+    torch.cuda.synchronize()
+    ins = [x * 1, x * 2]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(5):
+        for k, st in enumerate((s1, s2)):
+            with torch.cuda.stream(st):
+                got[k] = block(ins[k], dy)
+    torch.cuda.synchronize()
+    for a, c in zip(got, want):
+        assert all(torch.equal(p, r) for p, r in zip(a, c))
+
+
+def test_layer_norm_refuses_to_record_in_a_capture():
+    x = torch.randn(8, 16, device=DEV, requires_grad=True)
+    ops.layer_norm(x)
+    s = torch.zeros(1, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s.add_(1)
+        with pytest.raises(RuntimeError, match="during graph capture"):
+            ops.layer_norm(x)
+        with torch.no_grad():
+            y = ops.layer_norm(x)
+    graph.replay()
+    assert torch.equal(y, ops.layer_norm(x).detach())
+
+
+# ---- refusals ---------------------------------------------------------------------------------------------------------------
+def test_refusals():
+    x = torch.randn(4, 32, device=DEV)
+    lin = ops.LinearI8.quantize(torch.randn(8, 32, device=DEV))
+    q, s = ops.quantize_rows(x)
+    y, m, r = ops.layer_norm_forward(x)
+    for call, err in (
+            (lambda: ops.layer_norm(x.half()), TypeError), (lambda: ops.layer_norm(x.cpu()), RuntimeError),
+            (lambda: ops.layer_norm(x, torch.ones(31, device=DEV)), ValueError), (lambda: ops.layer_norm(x, torch.ones(32)), RuntimeError),
+            (lambda: ops.layer_norm(torch.randn(2, 8193, device=DEV)), RuntimeError), (lambda: ops.layer_norm(x, eps=-1.0), RuntimeError),
+            (lambda: ops.layer_norm(torch.randn(3, 0, device=DEV)), ValueError), (lambda: ops.layer_norm(torch.tensor(1.0, device=DEV)), ValueError),
+            (lambda: ops.layer_norm_backward(x.bfloat16(), x, m, r), ValueError), (lambda: ops.layer_norm_backward(x[:3], x, m, r), ValueError),
+            (lambda: ops.layer_norm_backward(x, x, m[:2], r), ValueError), (lambda: ops.quantize_rows(x.double()), TypeError),
+            (lambda: ops.matmul_i8(q, s, lin, act="relu6"), ValueError), (lambda: ops.matmul_i8(q[:, :16], s, lin), ValueError),
+            (lambda: ops.matmul_i8(q, s[:2], lin), ValueError), (lambda: ops.matmul_i8(q, s, lin, out_dtype=torch.float16), TypeError),
+            (lambda: ops.matmul_i8(q, s, lin, res=torch.zeros(4, 8, device=DEV)), ValueError), (lambda: ops.matmul_i8(x, s, lin), ValueError),
+            (lambda: ops.matmul_i8(q, s, lin, res=torch.zeros(4, 7, device=DEV, dtype=BF16)), ValueError),
+            (lambda: ops.linear_i8(x[:, :16], lin), ValueError), (lambda: ops.LinearI8(q, s.cpu()), RuntimeError),
+            (lambda: ops.LinearI8(q, s[:3]), ValueError), (lambda: ops.LinearI8.quantize(torch.randn(4, 4, 3, 3, device=DEV)), ValueError)):
+        with pytest.raises(err):
+            call()

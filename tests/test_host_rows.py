@@ -1,0 +1,106 @@
+"""CPU-side checks of the layer-norm and 8-bit entry points: struct layouts, workspace sizes, and that every bad argument is
+turned away before anything is launched (addresses here are numbers that nothing reads)."""
+import ctypes as C
+import os
+import subprocess
+
+import pytest
+import torch
+
+from helpers import ROOT
+from yolo_amd import _ffi, ops
+
+P = 1 << 20        # an aligned address
+
+
+def test_struct_layouts():
+    names = ("ydet_layer_norm_desc", "ydet_layer_norm_grad_desc", "ydet_quantize_desc", "ydet_matmul_i8_desc")
+    last = ("eps", "param_dtype", "eps", "out_dtype")
+    src = '#include <stddef.h>\n#include <stdio.h>\n#include "ydet.h"\nint main(){' + "".join(
+        f'printf("%zu %zu ", sizeof({n}), offsetof({n}, {f}));' for n, f in zip(names, last)) + "return 0;}"
+    exe = os.path.join(ROOT, "build", "abi_rows")
+    os.makedirs(os.path.dirname(exe), exist_ok=True)
+    subprocess.run(["gcc", "-x", "c", "-", "-I", os.path.join(ROOT, "include"), "-o", exe], input=src.encode(), check=True)
+    got = [int(v) for v in subprocess.run([exe], capture_output=True, check=True).stdout.split()]
+    mine = (_ffi.LayerNormDesc, _ffi.LayerNormGradDesc, _ffi.QuantizeDesc, _ffi.MatmulI8Desc)
+    assert got == [v for m, f in zip(mine, last) for v in (C.sizeof(m), getattr(m, f).offset)]
+
+
+def ln(**kw):
+    d = dict(x=P, y=P, gamma=P, beta=P, mean=None, rstd=None, rows=4, C=32, x_ld=32, x_coff=0, y_ld=32, y_coff=0, dtype=0, param_dtype=0,
+             eps=1e-5)
+    d.update(kw)
+    return _ffi.lib().ydet_layer_norm(_ffi.LayerNormDesc(**d), None)
+
+
+def grad(ws=P, ws_bytes=1 << 30, **kw):
+    d = dict(dy=P, x=P, dx=P, gamma=P, mean=P, rstd=P, dgamma=P, dbeta=P, rows=4, C=32, dy_ld=32, dy_coff=0, x_ld=32, x_coff=0, dx_ld=32,
+             dx_coff=0, dtype=0, param_dtype=0)
+    d.update(kw)
+    return _ffi.lib().ydet_layer_norm_backward(_ffi.LayerNormGradDesc(**d), ws, ws_bytes, None)
+
+
+def quant(**kw):
+    d = dict(x=P, q=P, scale=P, gamma=None, beta=None, rows=4, C=20, x_ld=20, x_coff=0, q_ld=32, dtype=0, param_dtype=0, normalize=0, eps=0.0)
+    d.update(kw)
+    return _ffi.lib().ydet_quantize_rows_i8(_ffi.QuantizeDesc(**d), None)
+
+
+def product(**kw):
+    d = dict(x=P, x_scale=P, w=P, w_scale=P, bias=P, res=None, y=P, rows=4, K=64, N=32, kp=64, n_pad=128, x_ld=64, x_coff=0, y_ld=32,
+             y_coff=0, res_ld=0, res_coff=0, act=0, slope=0.0, res_mode=0, out_dtype=1)
+    d.update(kw)
+    return _ffi.lib().ydet_matmul_i8(_ffi.MatmulI8Desc(**d), None)
+
+
+ARG, WS = -1, -3
+
+
+@pytest.mark.parametrize("call,kw,text", [
+    (ln, dict(x=None), "null"), (ln, dict(y=None), "null"), (ln, dict(rows=-1), "rows"), (ln, dict(rows=1 << 31), "rows"), (ln, dict(C=0), "C="),
+    (ln, dict(C=8193, x_ld=9000, y_ld=9000), "C="), (ln, dict(x_ld=31), "slice"), (ln, dict(y_coff=1), "slice"), (ln, dict(x_coff=-1), "slice"),
+    (ln, dict(dtype=2), "dtype"), (ln, dict(param_dtype=7), "dtype"), (ln, dict(eps=-1.0), "eps"), (ln, dict(eps=float("nan")), "eps"),
+    (ln, dict(mean=P), "together"), (ln, dict(x=P + 2), "misaligned"),
+    (grad, dict(x=None), "null"), (grad, dict(mean=None), "null"), (grad, dict(rows=-5), "rows"), (grad, dict(C=8193), "C="),
+    (grad, dict(dx_ld=16), "slice"), (grad, dict(dy_coff=3), "slice"), (grad, dict(dtype=5), "dtype"), (grad, dict(ws=None), "workspace"),
+    (grad, dict(dgamma=P + 1), "misaligned"),
+    (quant, dict(x=None), "null"), (quant, dict(scale=None), "null"), (quant, dict(q_ld=20), "q_ld"), (quant, dict(q_ld=16), "q_ld"),
+    (quant, dict(q=P + 8), "misaligned"), (quant, dict(C=21), "slice"), (quant, dict(normalize=1, eps=-1.0), "eps"), (quant, dict(rows=-1), "rows"),
+    (product, dict(x=None), "null"), (product, dict(x_scale=None), "null"), (product, dict(w=None), "null"), (product, dict(y=None), "null"),
+    (product, dict(res_mode=1, res_ld=32), "null"), (product, dict(res_mode=1, res=P, res_ld=31), "residual"), (product, dict(K=0), "K="),
+    (product, dict(K=131072, kp=131072, x_ld=131072), "K="), (product, dict(kp=96), "padded"), (product, dict(K=65, x_ld=80), "padded"),
+    (product, dict(n_pad=64), "padded"), (product, dict(N=129, y_ld=160), "padded"), (product, dict(x_ld=63), "slice"), (product, dict(y_coff=1), "slice"),
+    (product, dict(x_ld=(1 << 23) + 16), "x_ld"), (product, dict(out_dtype=2), "out_dtype"), (product, dict(act=3), "act"), (product, dict(res_mode=3), "act"),
+    (product, dict(w=P + 8), "alignment"), (product, dict(w_scale=P + 4), "alignment"), (product, dict(y=P + 1), "misaligned"),
+    (product, dict(rows=(1 << 31) - 1), "rows")])
+def test_bad_arguments(call, kw, text):
+    assert call(**kw) == ARG
+    assert text in _ffi.lib().ydet_last_error().decode()
+
+
+def test_workspace():
+    size = _ffi.lib().ydet_layer_norm_backward_workspace_bytes
+    assert size(-1, 32) == size(4, 0) == size(4, 8193) == 0
+    assert size(0, 32) == size(1, 32) == 2 * 32 * 4
+    for C_ in (1, 255, 2048, 8192):
+        sizes = [size(r, C_) for r in (1, 100, 10000, 1 << 20, (1 << 31) - 1)]
+        assert sizes == sorted(sizes) and sizes[-1] <= 1024 * 2 * C_ * 4
+    assert grad(ws_bytes=size(4, 32) - 4) == WS
+    assert "workspace" in _ffi.lib().ydet_last_error().decode()
+
+
+def test_nothing_to_do_is_no_error():
+    assert ln(rows=0, x=None, y=None) == 0
+    assert quant(rows=0, x=None, q=None, scale=None) == 0
+    assert product(rows=0, x=None, y=None) == 0
+    assert grad(dx=None, dgamma=None, dbeta=None, ws=None, ws_bytes=0) == 0
+    assert grad(rows=0, dgamma=None, dbeta=None, ws=None, ws_bytes=0) == 0
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.randn(3, 16)
+    for call in (lambda: ops.layer_norm(x), lambda: ops.layer_norm(x.requires_grad_(True)), lambda: ops.layer_norm_forward(x),
+                 lambda: ops.quantize_rows(x), lambda: ops.layer_norm_quantize(x), lambda: ops.LinearI8.quantize(x),
+                 lambda: ops.LinearI8(torch.zeros(2, 4, dtype=torch.int8), torch.ones(2))):
+        with pytest.raises(RuntimeError):
+            call()

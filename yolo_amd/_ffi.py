@@ -83,6 +83,34 @@ class PreprocDesc(C.Structure):
                 ("pad_value", C.c_int32 * 3), ("mean", C.c_float * 3), ("std", C.c_float * 3)]
 
 
+class LayerNormDesc(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("y", C.c_void_p), ("gamma", C.c_void_p), ("beta", C.c_void_p), ("mean", C.c_void_p),
+                ("rstd", C.c_void_p), ("rows", C.c_int64), ("C", C.c_int32), ("x_ld", C.c_int32), ("x_coff", C.c_int32),
+                ("y_ld", C.c_int32), ("y_coff", C.c_int32), ("dtype", C.c_int32), ("param_dtype", C.c_int32),
+                ("eps", C.c_float)]
+
+
+class LayerNormGradDesc(C.Structure):
+    _fields_ = [("dy", C.c_void_p), ("x", C.c_void_p), ("dx", C.c_void_p), ("gamma", C.c_void_p), ("mean", C.c_void_p),
+                ("rstd", C.c_void_p), ("dgamma", C.c_void_p), ("dbeta", C.c_void_p), ("rows", C.c_int64), ("C", C.c_int32),
+                ("dy_ld", C.c_int32), ("dy_coff", C.c_int32), ("x_ld", C.c_int32), ("x_coff", C.c_int32),
+                ("dx_ld", C.c_int32), ("dx_coff", C.c_int32), ("dtype", C.c_int32), ("param_dtype", C.c_int32)]
+
+
+class QuantizeDesc(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("q", C.c_void_p), ("scale", C.c_void_p), ("gamma", C.c_void_p), ("beta", C.c_void_p),
+                ("rows", C.c_int64), ("C", C.c_int32), ("x_ld", C.c_int32), ("x_coff", C.c_int32), ("q_ld", C.c_int32),
+                ("dtype", C.c_int32), ("param_dtype", C.c_int32), ("normalize", C.c_int32), ("eps", C.c_float)]
+
+
+class MatmulI8Desc(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("x_scale", C.c_void_p), ("w", C.c_void_p), ("w_scale", C.c_void_p), ("bias", C.c_void_p),
+                ("res", C.c_void_p), ("y", C.c_void_p), ("rows", C.c_int64), ("K", C.c_int32), ("N", C.c_int32),
+                ("kp", C.c_int32), ("n_pad", C.c_int32), ("x_ld", C.c_int32), ("x_coff", C.c_int32), ("y_ld", C.c_int32),
+                ("y_coff", C.c_int32), ("res_ld", C.c_int32), ("res_coff", C.c_int32), ("act", C.c_int32),
+                ("slope", C.c_float), ("res_mode", C.c_int32), ("out_dtype", C.c_int32)]
+
+
 class Op(C.Structure):
     _fields_ = [
         ("kind", C.c_int32), ("iarg", C.c_int32), ("iarg2", C.c_int32), ("iarg3", C.c_int32),
@@ -141,6 +169,11 @@ SYMBOLS = {
     "ydet_voc_match": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
                                  C.c_double, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "ydet_preprocess_u8": (C.c_int, [C.c_void_p, C.POINTER(PreprocDesc), C.c_void_p, C.c_void_p]),
+    "ydet_layer_norm": (C.c_int, [C.POINTER(LayerNormDesc), C.c_void_p]),
+    "ydet_layer_norm_backward_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int]),
+    "ydet_layer_norm_backward": (C.c_int, [C.POINTER(LayerNormGradDesc), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "ydet_quantize_rows_i8": (C.c_int, [C.POINTER(QuantizeDesc), C.c_void_p]),
+    "ydet_matmul_i8": (C.c_int, [C.POINTER(MatmulI8Desc), C.c_void_p]),
     "ydet_run_ops": (C.c_int, [C.POINTER(Op), C.c_int, C.c_void_p]),
     "ydet_run_op_lists": (C.c_int, [C.POINTER(C.POINTER(Op)), C.POINTER(C.c_int), C.c_int, C.c_void_p]),
     "ydet_timer_create": (C.c_void_p, [C.c_int]),

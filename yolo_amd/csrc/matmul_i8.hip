@@ -1,0 +1,383 @@
+// Product of rows held in 8 bits with weights held in 8 bits, a scale for every row and one for every output channel: the
+// 1x1 convolution (a token-wise linear layer) in 8-bit integers, with the epilogue of the floating convolutions.
+//
+//   acc[m, n] = sum_k x[m, k] w[n, k]   (32-bit integers: exact, whatever the order)
+//   y[m, n]   = act(acc * x_scale[m] * w_scale[n] + bias[n])  [+ res]          (or the residual before the activation)
+//
+// v_mfma_i32_16x16x64_i8: both operands are K-contiguous, a lane holds 16 consecutive k of one row.  Channels sit on the
+// MFMA row, pixels on its column, and weight rows are fetched in an order that leaves a lane with whole runs of
+// consecutive channels of one pixel, which it finishes and stores in 16-byte pieces.
+#include "conv_common.h"
+
+namespace ydet {
+namespace i8 {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+struct Args {
+    const char* x;          // first value of the slice
+    const float* xs;
+    const char* w;          // [n_pad][kp], zero behind K and N
+    const float* ws;        // n_pad values
+    const float* bias;      // n_pad values, or null
+    const char* res;
+    char* y;
+    int M, K, N, kp, n_pad;
+    long long x_ld, y_ld, res_ld;
+    int act, res_mode;
+    float slope;
+    int vec;                // 16-byte stores and residual loads are legal (and N is a multiple of the run of channels a lane holds)
+    int tiles_n;
+};
+
+__device__ __forceinline__ i32x4 mma(const i32x4& a, const i32x4& b, const i32x4& c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float finish(float v, float r, const Args& a) {
+    if (a.res_mode == YDET_RES_BEFORE_ACT) v += r;
+    v = conv::activate(v, a.act, a.slope);
+    return a.res_mode == YDET_RES_AFTER_ACT ? v + r : v;
+}
+
+// C consecutive channels n.. of pixel m: scales, bias, residual, activation, store.  C is 4, 8 or 16.
+template <typename OUT, int C>
+__device__ __forceinline__ void store_run(const Args& a, int m, int n, float xs, const int (&acc)[C]) {
+    constexpr int E = 16 / (int)sizeof(OUT);      // values of a 16-byte piece
+    typedef OUT piece __attribute__((ext_vector_type(E < C ? E : C)));
+    constexpr int PE = E < C ? E : C;
+    if (m >= a.M || n >= a.N) return;
+    float v[C];
+#pragma unroll
+    for (int i = 0; i < C; i += 4) {
+        const float4 s = *reinterpret_cast<const float4*>(a.ws + n + i);
+        const float4 b = a.bias ? *reinterpret_cast<const float4*>(a.bias + n + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[i] = fmaf((float)acc[i] * xs, s.x, b.x);
+        v[i + 1] = fmaf((float)acc[i + 1] * xs, s.y, b.y);
+        v[i + 2] = fmaf((float)acc[i + 2] * xs, s.z, b.z);
+        v[i + 3] = fmaf((float)acc[i + 3] * xs, s.w, b.w);
+    }
+    OUT* y = reinterpret_cast<OUT*>(a.y) + m * a.y_ld + n;
+    const OUT* res = a.res_mode == YDET_RES_NONE ? nullptr : reinterpret_cast<const OUT*>(a.res) + m * a.res_ld + n;
+    if (a.vec) {
+        piece r[C / PE];
+#pragma unroll
+        for (int p = 0; p < C / PE; ++p) r[p] = res ? *reinterpret_cast<const piece*>(res + p * PE) : piece{};
+#pragma unroll
+        for (int p = 0; p < C / PE; ++p) {
+            piece o;
+#pragma unroll
+            for (int e = 0; e < PE; ++e) o[e] = (OUT)finish(v[p * PE + e], (float)r[p][e], a);
+            *reinterpret_cast<piece*>(y + p * PE) = o;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+            if (n + i < a.N) y[i] = (OUT)finish(v[i], res ? (float)res[i] : 0.f, a);
+    }
+}
+
+// ---- tiles: BN channels x BM pixels, operands through LDS --------------------------------------------------------------
+// LDS image of a stage: BN weight rows, then BM pixel rows, 128 bytes of K each; row r's 16-byte piece c lies at place
+// c ^ ((r >> 1) & 7), so that the 16 rows a fragment read touches fall into 16 different places of the banks.  Stages are filled by
+// LDS-DMA (eight rows an instruction); rows behind the last pixel and channels behind n_pad lie outside the buffer
+// descriptors and read as zeros.  Two stages; the fragments of a half stage are read while the previous half's MFMAs run.
+template <typename OUT, int BN, int BM, int WAVES_N, int WAVES_M>
+__global__ __launch_bounds__(64 * WAVES_N * WAVES_M, 2) void tile_kernel(const Args a) {
+    constexpr int NW = WAVES_N * WAVES_M, WN = BN / WAVES_N, WM = BM / WAVES_M, FN = WN / 16, FM = WM / 16;
+    constexpr int RB = 128, STAGE = (BN + BM) * RB, LW = BN / 8 / NW, LX = BM / 8 / NW;
+    static_assert(WN % 64 == 0 && BN % (8 * NW) == 0 && BM % (8 * NW) == 0, "tile shape");
+    extern __shared__ __attribute__((aligned(128))) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wn = wave % WAVES_N, wm = wave / WAVES_N;
+    const unsigned t = xcd_remap(blockIdx.x, gridDim.x);
+    const int n0 = (int)(t % (unsigned)a.tiles_n) * BN, m0 = (int)(t / (unsigned)a.tiles_n) * BM;
+
+    const long long w_span = (long long)(a.n_pad - n0) * a.kp, x_span = (long long)(a.M - 1 - m0) * a.x_ld + ((a.K + 15) & ~15);
+    const unsigned cap = 0xffffffffu;
+    const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(a.w + (long long)n0 * a.kp), 0,
+                                                                        (int)(w_span < cap ? (unsigned)w_span : cap), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(a.x + m0 * a.x_ld), 0,
+                                                                        (int)(x_span < cap ? (unsigned)x_span : cap), 0x00020000);
+    unsigned ow[LW], ox[LX];
+#pragma unroll
+    for (int j = 0; j < LW; ++j) {
+        const int r = (j * NW + wave) * 8 + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
+        // LDS row (i, q, e) of a 64-channel group holds channel (q, i, e): fragment i, lane group q, register e
+        const int chan = (r & ~63) + ((r >> 2) & 3) * 16 + ((r >> 4) & 3) * 4 + (r & 3);
+        ow[j] = (unsigned)chan * (unsigned)a.kp + c * 16;
+    }
+#pragma unroll
+    for (int j = 0; j < LX; ++j) {
+        const int r = (j * NW + wave) * 8 + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
+        ox[j] = (unsigned)r * (unsigned)a.x_ld + c * 16;
+    }
+    auto issue = [&](int stage, int kt) {
+        char* dst = smem + stage * STAGE + wave * 1024;
+#pragma unroll
+        for (int j = 0; j < LW; ++j)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (__attribute__((address_space(3))) void*)(dst + j * NW * 1024), 16, (int)ow[j],
+                                                     kt * RB, 0, 0);
+#pragma unroll
+        for (int j = 0; j < LX; ++j)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (__attribute__((address_space(3))) void*)(dst + BN * RB + j * NW * 1024), 16,
+                                                     (int)ox[j], kt * RB, 0, 0);
+    };
+    int fo[2];
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) fo[kk] = (lane & 15) * RB + (((kk * 4 + (lane >> 4)) ^ ((lane & 15) >> 1)) * 16);
+    i32x4 fa[2][FN], fb[2][FM], acc[FN][FM];
+    auto read = [&](int stage, int kk, i32x4 (&A)[FN], i32x4 (&B)[FM]) {
+        const char* pw = smem + stage * STAGE + wn * WN * RB + fo[kk];
+        const char* px = smem + stage * STAGE + (BN + wm * WM) * RB + fo[kk];
+#pragma unroll
+        for (int i = 0; i < FN; ++i) A[i] = *reinterpret_cast<const i32x4*>(pw + i * 16 * RB);
+#pragma unroll
+        for (int j = 0; j < FM; ++j) B[j] = *reinterpret_cast<const i32x4*>(px + j * 16 * RB);
+    };
+    auto product = [&](const i32x4 (&A)[FN], const i32x4 (&B)[FM]) {
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int j = 0; j < FM; ++j) acc[i][j] = mma(A[i], B[j], acc[i][j]);
+    };
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+
+    const int halves = a.kp / 64, nk = (halves + 1) / 2;
+    issue(0, 0);
+    if (nk > 1) {
+        issue(1, 1);
+        conv::wait_vmcnt<LW + LX>();
+    } else {
+        conv::wait_vmcnt<0>();
+    }
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read(0, 0, fa[0], fb[0]);
+    // One stage: its second half is read under the first half's MFMAs; then every wave has its fragments and its own pieces
+    // of the next stage, the barrier makes both common, the stage is refilled and the next one's first half is read under the second
+    // half's MFMAs.  REFILL / MORE / WHOLE: a stage after the next, a next stage, a second half exist (compile-time, so
+    // that reads and MFMAs share a basic block).
+    auto stage_step = [&](auto refill, auto more, auto whole, int kt) {
+        constexpr bool REFILL = decltype(refill)::value, MORE = decltype(more)::value, WHOLE = decltype(whole)::value;
+        const int cur = kt & 1;
+        if constexpr (WHOLE) {
+            read(cur, 1, fa[1], fb[1]);
+            product(fa[0], fb[0]);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+#pragma unroll
+            for (int r = 0; r < FN + FM; ++r) {
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+            }
+            if constexpr (MORE) {
+                conv::wait_vmcnt<0>();
+                conv::wait_lgkmcnt<0>();
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                if constexpr (REFILL) issue(cur, kt + 2);
+                read(cur ^ 1, 0, fa[0], fb[0]);
+            }
+            product(fa[1], fb[1]);
+            if constexpr (MORE) {
+                if constexpr (REFILL) __builtin_amdgcn_sched_group_barrier(0x020, LW + LX, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+#pragma unroll
+                for (int r = 0; r < FN + FM; ++r) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+                }
+            }
+        } else {
+            product(fa[0], fb[0]);
+        }
+    };
+    constexpr std::true_type Y{};
+    constexpr std::false_type N{};
+    int kt = 0;
+    for (; kt + 2 < nk; ++kt) stage_step(Y, Y, Y, kt);
+    if (kt + 1 < nk) stage_step(N, Y, Y, kt++);
+    if (halves & 1) stage_step(N, N, N, kt);
+    else stage_step(N, N, Y, kt);
+
+    // lane (q, p): pixel p of every pixel fragment, channels 16 q .. + 15 of every 64-channel group
+    const int q = lane >> 4, p = lane & 15;
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+        const int m = m0 + wm * WM + j * 16 + p;
+        const float xs = m < a.M ? a.xs[m] : 0.f;
+#pragma unroll
+        for (int gI = 0; gI < FN / 4; ++gI) {
+            int v[16];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[i * 4 + e] = acc[gI * 4 + i][j][e];
+            store_run<OUT, 16>(a, m, n0 + wn * WN + gI * 64 + q * 16, xs, v);
+        }
+    }
+}
+
+// ---- few rows: the K of a small tile is shared by the waves of a workgroup ------------------------------------------------
+// 16 FN channels x 16 FM pixels a workgroup; each of its NW waves takes every NW-th 64 bytes of K, its operands straight
+// from memory into registers (all loads of a wave in flight together: the call costs one or two memory latencies), and the
+// waves' integer sums meet in LDS.  ANY: rows of x at any byte address and pitch (K need not be padded).
+template <bool ANY>
+__device__ __forceinline__ i32x4 load_k16(const char* p, int k, int K) {
+    if constexpr (!ANY) {
+        return k < K ? *reinterpret_cast<const i32x4*>(p + k) : i32x4{0, 0, 0, 0};
+    } else {
+        i32x4 v{0, 0, 0, 0};
+        if (k + 16 <= K) {
+            __builtin_memcpy(&v, p + k, 16);
+        } else if (k < K) {
+            unsigned u[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int i = 0; i < 15; ++i)
+                if (k + i < K) u[i >> 2] |= (unsigned)(unsigned char)p[k + i] << (8 * (i & 3));
+            v = i32x4{(int)u[0], (int)u[1], (int)u[2], (int)u[3]};
+        }
+        return v;
+    }
+}
+
+template <typename OUT, int FN, int FM, int NW, bool ANY>
+__global__ __launch_bounds__(64 * NW) void few_rows_kernel(const Args a) {
+    constexpr int AHEAD = 4;        // steps of K whose loads are in flight
+    __shared__ __attribute__((aligned(16))) i32x4 meet[NW][FN * FM][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, p = lane & 15;
+    const unsigned t = xcd_remap(blockIdx.x, gridDim.x);
+    const int n0 = (int)(t % (unsigned)a.tiles_n) * (16 * FN), m0 = (int)(t / (unsigned)a.tiles_n) * (16 * FM);
+    const char* pw[FN];
+    const char* px[FM];
+    // MFMA row (q, e) of fragment i is channel (q, i, e): a lane ends with 4 FN consecutive channels of its pixel
+#pragma unroll
+    for (int i = 0; i < FN; ++i) pw[i] = a.w + (long long)(n0 + (p >> 2) * (4 * FN) + i * 4 + (p & 3)) * a.kp;
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+        const int m = m0 + j * 16 + p;
+        px[j] = a.x + (long long)(m < a.M ? m : a.M - 1) * a.x_ld;
+    }
+    i32x4 acc[FN][FM];
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+    const int steps = a.kp / 64;
+    for (int s0 = wave; s0 < steps; s0 += NW * AHEAD) {
+        i32x4 fa[AHEAD][FN], fb[AHEAD][FM];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int s = s0 + u * NW, k = s * 64 + q * 16;
+            const bool in = s < steps;
+#pragma unroll
+            for (int i = 0; i < FN; ++i) fa[u][i] = in ? *reinterpret_cast<const i32x4*>(pw[i] + k) : i32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < FM; ++j) fb[u][j] = load_k16<ANY>(px[j], k, a.K);
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+            for (int i = 0; i < FN; ++i)
+#pragma unroll
+                for (int j = 0; j < FM; ++j) acc[i][j] = mma(fa[u][i], fb[u][j], acc[i][j]);
+    }
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j) meet[wave][j * FN + i][lane] = acc[i][j];
+    __syncthreads();
+    for (int j = wave; j < FM; j += NW) {
+        int v[4 * FN];
+#pragma unroll
+        for (int i = 0; i < FN; ++i) {
+            i32x4 s = meet[0][j * FN + i][lane];
+#pragma unroll
+            for (int k = 1; k < NW; ++k) s += meet[k][j * FN + i][lane];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i * 4 + e] = s[e];
+        }
+        const int m = m0 + j * 16 + p;
+        store_run<OUT, 4 * FN>(a, m, n0 + q * 4 * FN, m < a.M ? a.xs[m] : 0.f, v);
+    }
+}
+
+template <typename OUT, int BN, int BM, int WAVES_N, int WAVES_M>
+static int launch_tile(Args a, hipStream_t stream) {
+    constexpr int lds = 2 * (BN + BM) * 128;
+    a.tiles_n = (a.N + BN - 1) / BN;
+    const long long blocks = (long long)a.tiles_n * ((a.M + BM - 1) / BM);
+    YDET_CHECK_ARG(blocks * 64 * WAVES_N * WAVES_M <= UINT32_MAX, "matmul_i8: %d rows x %d channels are too many tiles", a.M, a.N);
+    static unsigned char done[kMaxDevices];
+    const int rc = raise_dynamic_lds_limit(reinterpret_cast<const void*>(&tile_kernel<OUT, BN, BM, WAVES_N, WAVES_M>), lds, done, "matmul_i8");
+    if (rc != YDET_OK) return rc;
+    hipLaunchKernelGGL((tile_kernel<OUT, BN, BM, WAVES_N, WAVES_M>), dim3((unsigned)blocks), dim3(64 * WAVES_N * WAVES_M), lds, stream, a);
+    YDET_CHECK_LAUNCH("matmul_i8");
+    return YDET_OK;
+}
+
+template <typename OUT, int FN, int FM, int NW, bool ANY>
+static int launch_few(Args a, hipStream_t stream) {
+    a.tiles_n = (a.N + 16 * FN - 1) / (16 * FN);
+    const long long blocks = (long long)a.tiles_n * ((a.M + 16 * FM - 1) / (16 * FM));
+    YDET_CHECK_ARG(blocks * 64 * NW <= UINT32_MAX, "matmul_i8: %d rows x %d channels are too many tiles", a.M, a.N);
+    hipLaunchKernelGGL((few_rows_kernel<OUT, FN, FM, NW, ANY>), dim3((unsigned)blocks), dim3(64 * NW), 0, stream, a);
+    YDET_CHECK_LAUNCH("matmul_i8 (few rows)");
+    return YDET_OK;
+}
+
+template <typename OUT>
+static int launch(const Args& a, bool wide_x, hipStream_t stream) {
+    if (!wide_x) return a.M <= 16 ? launch_few<OUT, 1, 1, 8, true>(a, stream) : launch_few<OUT, 2, 2, 8, true>(a, stream);
+    const long long t128 = (long long)((a.M + 127) / 128) * ((a.N + 127) / 128);
+    if (a.M <= 16) return launch_few<OUT, 1, 1, 8, false>(a, stream);
+    if (t128 < current_device_info().cus / 2) return launch_few<OUT, 2, 2, 8, false>(a, stream);
+    return launch_tile<OUT, 128, 128, 2, 2>(a, stream);
+}
+
+}  // namespace i8
+}  // namespace ydet
+
+using namespace ydet;
+
+int ydet_launch_matmul_i8(const ydet_matmul_i8_desc* d, hipStream_t stream) {
+    YDET_CHECK_ARG(d, "matmul_i8: null descriptor");
+    YDET_CHECK_ARG(d->rows >= 0 && d->rows <= INT32_MAX - 512 && d->K > 0 && d->K <= 131071 && d->N > 0 && d->N <= (1 << 24),
+                   "matmul_i8: rows=%lld K=%d N=%d (K up to 131071: the sums are 32-bit integers)", (long long)d->rows, d->K, d->N);
+    YDET_CHECK_ARG(d->kp % 64 == 0 && d->kp >= d->K && d->n_pad % 128 == 0 && d->n_pad >= d->N,
+                   "matmul_i8: weights padded to %d x %d (want a multiple of 128 >= %d, a multiple of 64 >= %d)", d->n_pad, d->kp, d->N, d->K);
+    YDET_CHECK_ARG(d->x_coff >= 0 && d->y_coff >= 0 && (long long)d->x_coff + d->K <= d->x_ld && (long long)d->y_coff + d->N <= d->y_ld,
+                   "matmul_i8: a slice lies outside its rows");
+    YDET_CHECK_ARG(d->x_ld <= (1 << 23), "matmul_i8: x_ld=%d (up to %d)", d->x_ld, 1 << 23);
+    YDET_CHECK_ARG(d->out_dtype == YDET_F32 || d->out_dtype == YDET_BF16, "matmul_i8: out_dtype %d", d->out_dtype);
+    YDET_CHECK_ARG(d->act >= YDET_ACT_NONE && d->act <= YDET_ACT_SILU && d->res_mode >= YDET_RES_NONE && d->res_mode <= YDET_RES_BEFORE_ACT,
+                   "matmul_i8: act %d res_mode %d", d->act, d->res_mode);
+    YDET_CHECK_ARG(d->res_mode == YDET_RES_NONE || (d->res_coff >= 0 && (long long)d->res_coff + d->N <= d->res_ld),
+                   "matmul_i8: the residual's slice lies outside its rows");
+    if (d->rows == 0) return YDET_OK;
+    YDET_CHECK_ARG(d->x && d->x_scale && d->w && d->w_scale && d->y && (d->res_mode == YDET_RES_NONE || d->res), "matmul_i8: null pointer");
+    YDET_CHECK_ARG(((uintptr_t)d->w | (uintptr_t)d->w_scale | (uintptr_t)d->bias) % 16 == 0, "matmul_i8: weights, scales and bias need 16-byte alignment");
+    const size_t es = dtype_size(d->out_dtype);
+    i8::Args a{};
+    a.x = reinterpret_cast<const char*>(d->x) + d->x_coff;
+    a.xs = d->x_scale, a.w = reinterpret_cast<const char*>(d->w), a.ws = d->w_scale, a.bias = d->bias;
+    a.y = static_cast<char*>(d->y) + d->y_coff * es;
+    a.res_mode = d->res_mode;
+    if (a.res_mode != YDET_RES_NONE) a.res = static_cast<const char*>(d->res) + d->res_coff * es;
+    YDET_CHECK_ARG(((uintptr_t)a.y | (uintptr_t)a.res) % es == 0 && (uintptr_t)a.xs % 4 == 0, "matmul_i8: misaligned tensor");
+    a.M = (int)d->rows, a.K = d->K, a.N = d->N, a.kp = d->kp, a.n_pad = d->n_pad;
+    a.x_ld = d->x_ld, a.y_ld = d->y_ld, a.res_ld = d->res_ld, a.act = d->act, a.slope = d->slope;
+    auto wide = [&](const char* p, int ld) { return (uintptr_t)p % 16 == 0 && ld * es % 16 == 0; };
+    a.vec = d->N % 16 == 0 && wide(a.y, d->y_ld) && (a.res_mode == YDET_RES_NONE || wide(a.res, d->res_ld));
+    // rows read in 16-byte pieces: the last piece of a row may reach behind K, so the pitch has to hold it
+    const bool wide_x = (uintptr_t)a.x % 16 == 0 && d->x_ld % 16 == 0 && d->x_coff + (d->K + 15) / 16 * 16 <= d->x_ld;
+    return d->out_dtype == YDET_BF16 ? i8::launch<__bf16>(a, wide_x, stream) : i8::launch<float>(a, wide_x, stream);
+}
+
+extern "C" int ydet_matmul_i8(const ydet_matmul_i8_desc* d, void* stream) {
+    clear_error();
+    return ydet_launch_matmul_i8(d, as_stream(stream));
+}

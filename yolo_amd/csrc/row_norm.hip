@@ -1,0 +1,277 @@
+// Layer normalisation over channels and symmetric 8-bit quantisation of rows, each alone or the second behind the first, on
+// NHWC slices: a row is the C channels of one pixel.
+//
+//   norm      mu = sum_c x_c / C,  var = sum_c (x_c - mu)^2 / C,  r = 1 / sqrt(var + eps),  y_c = (x_c - mu) * r * w_c + b_c
+//   quantise  s = max_c |y_c| / 127 (rounded once),  q_c = the integer nearest y_c / s, ties to even
+//
+// One pass over memory: a row is read once into the registers of the lanes that share it (rows_common.h), mean, variance
+// (from the differences to the mean, not as a difference of squares) and maximum are taken there, and the result is
+// written.  About ten operations a value against two to eight bytes: bound by HBM.  Sums, statistics and scales are in 32 bits.
+#include "rows_common.h"
+
+namespace ydet {
+namespace rows {
+
+struct RowArgs {
+    const char* x;      // first value of the slice
+    char* y;            // normalised rows, or 8-bit rows
+    float* scale;
+    const char* gamma;
+    const char* beta;
+    float* mean;
+    float* rstd;
+    long long rows;
+    int C, cw;          // values of a row; values written of a row (8-bit rows: zeros behind C)
+    int x_ld, y_ld;
+    int param_dtype;
+    float eps;
+};
+
+enum { kNorm = 1, kQuant = 2 };
+
+// Nearest integer to v / s (ties to even), exactly, as a float's bits whose low byte is the integer.  The product with 1 / s
+// is within 3e-5 of the quotient, so rounding it (adding 1.5 * 2^23 leaves the integer in the low bits) is right unless it
+// lies that close to a border; there the remainder decides, which the fused multiply-add gives without error: near a
+// border |v - r s| is about s / 2 and a multiple of s's last place.
+__device__ __forceinline__ unsigned quantise_exact(float v, float s, float inv) {
+    constexpr float kMagic = 12582912.f;
+    float r = (v * inv + kMagic) - kMagic;
+    const float d = fmaf(-r, s, v), d2 = 2.f * fabsf(d);
+    if (d2 > s || (d2 == s && ((int)r & 1))) r += copysignf(1.f, d);
+    return __float_as_uint(r + kMagic);
+}
+
+template <int MODE, typename T, bool RAG, int LPR, int CH, int RPT>
+__global__ __launch_bounds__(kThreads) void row_norm_kernel(const RowArgs a) {
+    constexpr int VEC = 16 / (int)sizeof(T);
+    using P = Piece<T, VEC, RAG>;
+    constexpr int G = kThreads / LPR;       // rows of a workgroup at a time
+    constexpr bool NORM = (MODE & kNorm) != 0, QUANT = (MODE & kQuant) != 0;
+    __shared__ unsigned red[2][4];
+    int slot = 0;
+    const int tid = threadIdx.x, g = tid / LPR, l = tid % LPR;
+    const float fc = (float)a.C;
+    float w[NORM ? CH * VEC : 1], b[NORM ? CH * VEC : 1];
+    if constexpr (NORM) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int col = (c * LPR + l) * VEC;
+            load_params<VEC, RAG>(a.gamma, a.param_dtype, col, a.C - col, 1.f, w + c * VEC);
+            load_params<VEC, RAG>(a.beta, a.param_dtype, col, a.C - col, 0.f, b + c * VEC);
+        }
+    }
+    for (long long row0 = (long long)blockIdx.x * (G * RPT); row0 < a.rows; row0 += (long long)gridDim.x * (G * RPT)) {
+        typename P::type in[RPT][CH];
+#pragma unroll
+        for (int r = 0; r < RPT; ++r) {
+            const long long row = row0 + r * G + g;
+            const T* xr = reinterpret_cast<const T*>(a.x) + row * a.x_ld;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const int col = (c * LPR + l) * VEC;
+                in[r][c] = typename P::type{};
+                if (row < a.rows && col < a.C) in[r][c] = P::load(xr + col, a.C - col);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < RPT; ++r) {
+            const long long row = row0 + r * G + g;
+            const bool live = row < a.rows;
+            float v[CH * VEC];
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) v[c * VEC + i] = (float)in[r][c][i];
+            if constexpr (NORM) {
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < CH * VEC; ++i) sum += v[i];
+                const float mean = group_sum<LPR>(sum, red, slot) / fc;
+                float sq = 0.f;
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    const int left = a.C - (c * LPR + l) * VEC;
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        const float d = P::has(i, left) ? v[c * VEC + i] - mean : 0.f;
+                        v[c * VEC + i] = d;
+                        sq = fmaf(d, d, sq);
+                    }
+                }
+                const float rstd = 1.f / sqrtf(group_sum<LPR>(sq, red, slot) / fc + a.eps);
+                if (a.mean && live && l == 0) {
+                    a.mean[row] = mean;
+                    a.rstd[row] = rstd;
+                }
+#pragma unroll
+                for (int i = 0; i < CH * VEC; ++i) v[i] = P::has(i % VEC, a.C - (i / VEC * LPR + l) * VEC) ? fmaf(v[i] * rstd, w[i], b[i]) : 0.f;
+            }
+            if constexpr (!QUANT) {
+                if (live) {
+                    T* yr = reinterpret_cast<T*>(a.y) + row * a.y_ld;
+#pragma unroll
+                    for (int c = 0; c < CH; ++c) {
+                        const int col = (c * LPR + l) * VEC;
+                        if (col < a.C) {
+                            typename P::type o;
+#pragma unroll
+                            for (int i = 0; i < VEC; ++i) o[i] = (T)v[c * VEC + i];
+                            P::store(yr + col, o, a.C - col);
+                        }
+                    }
+                }
+            } else {
+                // largest magnitude by its bits: a NaN is above an infinity, and that above every number.  (Lanes and pieces
+                // behind the row's end hold zeros.)
+                unsigned top = 0;
+#pragma unroll
+                for (int i = 0; i < CH * VEC; ++i) {
+                    const unsigned u = __float_as_uint(v[i]) & 0x7fffffffu;
+                    top = u > top ? u : top;
+                }
+                top = group_reduce<LPR>(top, MaxU{}, red, slot);
+                const float amax = __uint_as_float(top);
+                const bool bad = top >= 0x7f800000u;                 // the row has no scale: NaN, and zeros
+                const bool some = !bad && amax >= 127.f * 1.17549435e-38f;   // smaller rows count as zero: s stays a normal number
+                const float s = some ? amax / 127.f : 1.f, inv = 1.f / s;
+                if (live && l == 0) a.scale[row] = some ? s : bad ? __uint_as_float(0x7fc00000u) : 0.f;
+                unsigned m[CH * VEC];
+                float near = 0.f;
+#pragma unroll
+                for (int i = 0; i < CH * VEC; ++i) {
+                    constexpr float kMagic = 12582912.f;
+                    v[i] = some ? v[i] : 0.f;
+                    const float t = v[i] * inv, k = t + kMagic;
+                    near = fmaxf(near, fabsf(t - (k - kMagic)));
+                    m[i] = __float_as_uint(k);
+                }
+                if (near > 0.4999f) {
+#pragma unroll
+                    for (int i = 0; i < CH * VEC; ++i) m[i] = quantise_exact(v[i], s, inv);
+                }
+                if (live) {
+                    char* yr = a.y + row * a.y_ld;
+#pragma unroll
+                    for (int c = 0; c < CH; ++c) {
+                        const int col = (c * LPR + l) * VEC;
+                        if (col < a.cw) {
+                            unsigned d[VEC / 4];
+#pragma unroll
+                            for (int j = 0; j < VEC / 4; ++j) {
+                                const unsigned lo = __builtin_amdgcn_perm(m[c * VEC + 4 * j + 1], m[c * VEC + 4 * j], 0x0c0c0400u);
+                                const unsigned hi = __builtin_amdgcn_perm(m[c * VEC + 4 * j + 3], m[c * VEC + 4 * j + 2], 0x0c0c0400u);
+                                d[j] = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+                            }
+                            if constexpr (VEC == 8) *reinterpret_cast<uint2*>(yr + col) = make_uint2(d[0], d[1]);
+                            else *reinterpret_cast<unsigned*>(yr + col) = d[0];
+                        }
+                    }
+                }
+            }
+        }
+    }
+}
+
+template <int MODE, typename T, bool RAG, int LPR, int CH, int RPT>
+static int launch_rows(const RowArgs& a, hipStream_t stream) {
+    constexpr int per = kThreads / LPR * RPT;
+    const long long need = (a.rows + per - 1) / per;
+    const unsigned blocks = (unsigned)(need < (1 << 20) ? need : (1 << 20));
+    hipLaunchKernelGGL((row_norm_kernel<MODE, T, RAG, LPR, CH, RPT>), dim3(blocks), dim3(kThreads), 0, stream, a);
+    YDET_CHECK_LAUNCH("row norm / quantise");
+    return YDET_OK;
+}
+
+// Rows a lane group takes at once: four (their loads in flight together, weight and bias read once for them) where that still
+// leaves eight workgroups a CU, else one.
+template <int MODE, typename T, bool RAG, int LPR, int CH>
+static int launch_depth(const RowArgs& a, hipStream_t stream) {
+    if constexpr (CH == 1) {
+        if (a.rows >= (long long)current_device_info().cus * 8 * 4 * (kThreads / LPR))
+            return launch_rows<MODE, T, RAG, LPR, CH, 4>(a, stream);
+    }
+    return launch_rows<MODE, T, RAG, LPR, CH, 1>(a, stream);
+}
+
+template <int MODE, typename T, bool RAG>
+static int launch_shape(const RowArgs& a, hipStream_t stream) {
+    const Shape s = shape_of(a.cw, 16 / (int)sizeof(T));
+#define YDET_ROWS(L, K) \
+    if (s.lpr == L && s.ch == K) return launch_depth<MODE, T, RAG, L, K>(a, stream);
+    YDET_ROWS(4, 1) YDET_ROWS(8, 1) YDET_ROWS(16, 1) YDET_ROWS(32, 1) YDET_ROWS(64, 1) YDET_ROWS(64, 2) YDET_ROWS(64, 4) YDET_ROWS(256, 4)
+    if constexpr (sizeof(T) == 4) {
+        YDET_ROWS(64, 8) YDET_ROWS(256, 8)
+    } else {
+        YDET_ROWS(256, 2)
+    }
+#undef YDET_ROWS
+    return fail(YDET_ERR_ARG, "row norm: no kernel for %d channels", a.C);
+}
+
+template <int MODE>
+static int launch_mode(const RowArgs& a, int dtype, hipStream_t stream) {
+    if (dtype == YDET_BF16) return a.C % 8 ? launch_shape<MODE, __bf16, true>(a, stream) : launch_shape<MODE, __bf16, false>(a, stream);
+    return a.C % 4 ? launch_shape<MODE, float, true>(a, stream) : launch_shape<MODE, float, false>(a, stream);
+}
+
+}  // namespace rows
+}  // namespace ydet
+
+using namespace ydet;
+using namespace ydet::rows;
+
+int ydet_launch_layer_norm(const ydet_layer_norm_desc* d, hipStream_t stream) {
+    YDET_CHECK_ARG(d, "layer_norm: null descriptor");
+    YDET_CHECK_ARG(d->rows >= 0 && d->rows <= INT32_MAX && d->C > 0 && d->C <= kMaxC, "layer_norm: rows=%lld C=%d (C 1..%d)",
+                   (long long)d->rows, d->C, kMaxC);
+    YDET_CHECK_ARG(dtype_ok(d->dtype) && dtype_ok(d->param_dtype), "layer_norm: dtype %d / %d", d->dtype, d->param_dtype);
+    YDET_CHECK_ARG(d->x_coff >= 0 && d->y_coff >= 0 && (long long)d->x_coff + d->C <= d->x_ld && (long long)d->y_coff + d->C <= d->y_ld,
+                   "layer_norm: slice of %d channels at %d / %d outside rows of %d / %d", d->C, d->x_coff, d->y_coff, d->x_ld, d->y_ld);
+    YDET_CHECK_ARG(d->eps >= 0.f, "layer_norm: eps=%g", (double)d->eps);
+    YDET_CHECK_ARG(!d->mean == !d->rstd, "layer_norm: mean and rstd come together");
+    if (d->rows == 0) return YDET_OK;
+    YDET_CHECK_ARG(d->x && d->y, "layer_norm: null pointer");
+    const size_t es = dtype_size(d->dtype);
+    RowArgs a{};
+    a.x = static_cast<const char*>(d->x) + d->x_coff * es;
+    a.y = static_cast<char*>(d->y) + d->y_coff * es;
+    YDET_CHECK_ARG(((uintptr_t)a.x | (uintptr_t)a.y) % es == 0, "layer_norm: misaligned tensor");
+    a.gamma = static_cast<const char*>(d->gamma), a.beta = static_cast<const char*>(d->beta);
+    a.mean = d->mean, a.rstd = d->rstd, a.rows = d->rows, a.C = a.cw = d->C;
+    a.x_ld = d->x_ld, a.y_ld = d->y_ld, a.param_dtype = d->param_dtype, a.eps = d->eps;
+    return launch_mode<kNorm>(a, d->dtype, stream);
+}
+
+int ydet_launch_quantize_rows(const ydet_quantize_desc* d, hipStream_t stream) {
+    YDET_CHECK_ARG(d, "quantize_rows: null descriptor");
+    YDET_CHECK_ARG(d->rows >= 0 && d->rows <= INT32_MAX && d->C > 0 && d->C <= kMaxC, "quantize_rows: rows=%lld C=%d (C 1..%d)",
+                   (long long)d->rows, d->C, kMaxC);
+    YDET_CHECK_ARG(dtype_ok(d->dtype) && dtype_ok(d->param_dtype), "quantize_rows: dtype %d / %d", d->dtype, d->param_dtype);
+    const int cw = (d->C + 15) / 16 * 16;
+    YDET_CHECK_ARG(d->x_coff >= 0 && (long long)d->x_coff + d->C <= d->x_ld, "quantize_rows: slice of %d channels at %d outside rows of %d",
+                   d->C, d->x_coff, d->x_ld);
+    YDET_CHECK_ARG(d->q_ld >= cw && d->q_ld % 16 == 0, "quantize_rows: rows of %d channels need q_ld >= %d, a multiple of 16 (got %d)", d->C,
+                   cw, d->q_ld);
+    YDET_CHECK_ARG(!d->normalize || d->eps >= 0.f, "quantize_rows: eps=%g", (double)d->eps);
+    if (d->rows == 0) return YDET_OK;
+    YDET_CHECK_ARG(d->x && d->q && d->scale, "quantize_rows: null pointer");
+    const size_t es = dtype_size(d->dtype);
+    RowArgs a{};
+    a.x = static_cast<const char*>(d->x) + d->x_coff * es;
+    a.y = reinterpret_cast<char*>(d->q);
+    YDET_CHECK_ARG((uintptr_t)a.x % es == 0 && (uintptr_t)a.y % 16 == 0, "quantize_rows: misaligned tensor");
+    a.scale = d->scale, a.rows = d->rows, a.C = d->C, a.cw = cw, a.x_ld = d->x_ld, a.y_ld = d->q_ld;
+    a.gamma = static_cast<const char*>(d->gamma), a.beta = static_cast<const char*>(d->beta);
+    a.param_dtype = d->param_dtype, a.eps = d->eps;
+    return d->normalize ? launch_mode<kNorm | kQuant>(a, d->dtype, stream) : launch_mode<kQuant>(a, d->dtype, stream);
+}
+
+extern "C" int ydet_layer_norm(const ydet_layer_norm_desc* d, void* stream) {
+    clear_error();
+    return ydet_launch_layer_norm(d, as_stream(stream));
+}
+
+extern "C" int ydet_quantize_rows_i8(const ydet_quantize_desc* d, void* stream) {
+    clear_error();
+    return ydet_launch_quantize_rows(d, as_stream(stream));
+}

@@ -1,0 +1,132 @@
+// Pieces shared by the kernels that work row by row over channels (row_norm.hip, row_norm_grad.hip).  gfx950 only.
+#pragma once
+#include "ydet_internal.h"
+
+namespace ydet {
+namespace rows {
+
+// A row of C values is held in registers by LPR lanes (a power of two: a part of a wave, a wave, or the 256 lanes of a
+// workgroup), CH pieces of VEC values each; piece c of lane l starts at column (c * LPR + l) * VEC.  At most 32 values a lane:
+// rows up to 2048 values stay inside one wave, up to kMaxC inside one workgroup.
+constexpr int kMaxC = 8192;
+constexpr int kThreads = 256;
+
+struct Shape {
+    int lpr, ch;
+};
+static inline int pow2_at_least(int v) {
+    int p = 1;
+    while (p < v) p *= 2;
+    return p;
+}
+// cols: values of a row that are read or written; vec: values of a 16-byte piece (8 or 4)
+static inline Shape shape_of(int cols, int vec) {
+    const int n = (cols + vec - 1) / vec;
+    if (n <= 64) {
+        const int l = pow2_at_least(n);
+        return Shape{l < 4 ? 4 : l, 1};
+    }
+    if (n * vec <= 2048) return Shape{64, pow2_at_least((n + 63) / 64)};
+    const int least = vec == 4 ? 4 : 2, c = pow2_at_least((n + 255) / 256);
+    return Shape{256, c < least ? least : c};
+}
+
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp(unsigned v) {
+    return (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
+}
+// Combines the LPR <= 64 lanes of a group so that every lane holds the result; op is commutative and the tree is the same for
+// every lane, so all lanes hold the same bits.  Neighbours by DPP inside 16 lanes, then by the lane-row swaps.
+template <int LPR, typename F>
+__device__ __forceinline__ unsigned lanes_reduce(unsigned v, F op) {
+    if constexpr (LPR >= 2) v = op(v, dpp<0xB1>(v));       // quad_perm [1,0,3,2]
+    if constexpr (LPR >= 4) v = op(v, dpp<0x4E>(v));       // quad_perm [2,3,0,1]
+    if constexpr (LPR >= 8) v = op(v, dpp<0x141>(v));      // row_half_mirror
+    if constexpr (LPR >= 16) v = op(v, dpp<0x140>(v));     // row_mirror
+    if constexpr (LPR >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = op(r[0], r[1]);
+    }
+    if constexpr (LPR >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = op(r[0], r[1]);
+    }
+    return v;
+}
+struct AddF {
+    __device__ __forceinline__ unsigned operator()(unsigned a, unsigned b) const {
+        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+    }
+};
+struct MaxU {
+    __device__ __forceinline__ unsigned operator()(unsigned a, unsigned b) const { return a > b ? a : b; }
+};
+// The same over a group of LPR lanes where LPR may be the whole workgroup: its four waves meet in LDS.  `red` has two slots
+// of four words used in turn: a wave that writes a slot again has passed the barrier of the other one, which every wave
+// reaches only after it has read this one.
+template <int LPR, typename F>
+__device__ __forceinline__ unsigned group_reduce(unsigned v, F op, unsigned (&red)[2][4], int& slot) {
+    if constexpr (LPR <= 64) {
+        return lanes_reduce<LPR>(v, op);
+    } else {
+        v = lanes_reduce<64>(v, op);
+        if ((threadIdx.x & 63) == 0) red[slot][threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = op(op(red[slot][0], red[slot][1]), op(red[slot][2], red[slot][3]));
+        slot ^= 1;
+        return v;
+    }
+}
+template <int LPR>
+__device__ __forceinline__ float group_sum(float v, unsigned (&red)[2][4], int& slot) {
+    return __uint_as_float(group_reduce<LPR>(__float_as_uint(v), AddF{}, red, slot));
+}
+
+// A piece: VEC consecutive values, 16 bytes.  Rows may begin at any value's address (gfx950 moves 16 bytes from and to any
+// address), so a row is dealt to the lanes the same way wherever it lies, and its result does not depend on that.  RAG: C is no
+// multiple of VEC, and the row's last piece, `n` < VEC values of it, is moved value by value (zeros behind it).
+template <typename T, int VEC, bool RAG>
+struct Piece {
+    typedef T type __attribute__((ext_vector_type(VEC)));
+    typedef type loose __attribute__((aligned(sizeof(T))));
+    static __device__ __forceinline__ type load(const T* p, int n) {
+        if (!RAG || n >= VEC) return *reinterpret_cast<const loose*>(p);
+        type v{};
+#pragma unroll
+        for (int i = 0; i < VEC - 1; ++i)
+            if (i < n) v[i] = p[i];
+        return v;
+    }
+    static __device__ __forceinline__ void store(T* p, const type& v, int n) {
+        if (!RAG || n >= VEC) {
+            *reinterpret_cast<loose*>(p) = v;
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < VEC - 1; ++i)
+            if (i < n) p[i] = v[i];
+    }
+    // whether value i of a piece with n values of the row left is one of them
+    static __device__ __forceinline__ bool has(int i, int n) { return RAG ? i < n : n > 0; }
+};
+
+// The per-channel parameters (weight or bias) of a piece, of either type: `none` where there are none, zeros behind the row
+template <int VEC, bool RAG>
+__device__ __forceinline__ void load_params(const char* p, int dtype, int col, int n, float none, float* out) {
+    if (dtype == YDET_BF16) {
+        typedef Piece<__bf16, VEC, RAG> P;
+        typename P::type v{};
+        if (p && n > 0) v = P::load(reinterpret_cast<const __bf16*>(p) + col, n);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) out[i] = !P::has(i, n) ? 0.f : p ? (float)v[i] : none;
+    } else {
+        typedef Piece<float, VEC, RAG> P;
+        typename P::type v{};
+        if (p && n > 0) v = P::load(reinterpret_cast<const float*>(p) + col, n);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) out[i] = !P::has(i, n) ? 0.f : p ? v[i] : none;
+    }
+}
+
+}  // namespace rows
+}  // namespace ydet

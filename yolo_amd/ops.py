@@ -1,4 +1,4 @@
-"""Tensor-level wrappers of the decode / NMS / IoU entry points of libydet.so.
+"""Tensor-level wrappers of the decode / NMS / IoU, layer-norm and 8-bit entry points of libydet.so.
 
 Inputs and outputs are CUDA tensors; everything is enqueued on torch's current stream and nothing
 here synchronises with the host.
@@ -279,3 +279,256 @@ def voc_match(boxes, members, group_start, gt_boxes, gt_difficult, gt_start, ovt
                                       flags.data_ptr(), ws.data_ptr(), ws.numel() * 8, _ffi.current_stream()),
                    "ydet_voc_match")
     return flags
+
+
+# ---- operators over the channels of every pixel ----------------------------------------------------------------------
+# Tensors are [..., C]: any leading dimensions, the channels last (an NHWC map, or a channel slice of one).  Rows at one
+# common distance are read where they lie; other strides, and types other than fp32 / bf16, are copied or refused.
+MAX_ROW = 8192      # channels of a row that layer_norm and quantize_rows take
+
+
+def _launch(dev, call, *args):
+    """`call(*args, stream)` on torch's current stream of `dev`."""
+    if torch.cuda.current_device() == dev.index:
+        return call(*args, torch.cuda.current_stream().cuda_stream)
+    with torch.cuda.device(dev):
+        return call(*args, torch.cuda.current_stream().cuda_stream)
+
+
+def _as_rows(t, what):
+    """(t or a copy, rows, distance of rows) of a [..., C] tensor."""
+    if t.dim() == 0 or t.shape[-1] == 0:
+        raise ValueError(f"{what} needs at least one channel (shape {tuple(t.shape)})")
+    C = t.shape[-1]
+    n = t.numel() // C
+    if t.is_contiguous():
+        return t, n, C
+    if t.stride(-1) == 1 or C == 1:
+        try:
+            ld = t.view(-1, C).stride(0) if n > 1 else C
+        except RuntimeError:
+            ld = 0
+        if C <= ld < 2 ** 31 and (C > 1 or n == 1 or ld >= 1):
+            return t, n, ld
+    return t.contiguous(), n, C
+
+
+def _params(C, dev, *ps):
+    """The per-channel parameters (None allowed) as contiguous tensors of one type, and that type."""
+    dts = set()
+    for p in ps:
+        if p is None:
+            continue
+        if p.shape != (C,):
+            raise ValueError(f"weight and bias have one value a channel: got {tuple(p.shape)} for {C} channels")
+        if p.device != dev:
+            raise RuntimeError(f"weight / bias on {p.device}, the input on {dev}")
+        dts.add(_dt(p))
+    dt = _ffi.F32 if len(dts) != 1 else dts.pop()
+    td = torch.float32 if dt == _ffi.F32 else torch.bfloat16
+    return [p if p is None else p.detach().to(td).contiguous() for p in ps], dt
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, stats=True):
+    """Layer normalisation over the last dimension: (y, mean, rstd), y of x's dtype and shape, mean and rstd fp32 of
+    x.shape[:-1] (None without `stats`).  weight, bias: [C] fp32 or bf16, or None."""
+    _need_cuda(x)
+    lib = _ffi.lib()
+    dt = _dt(x)
+    x, n, ld = _as_rows(x, "layer_norm")
+    C = x.shape[-1]
+    (w, b), pdt = _params(C, x.device, weight, bias)
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    mean = torch.empty(x.shape[:-1], device=x.device) if stats else None
+    rstd = torch.empty(x.shape[:-1], device=x.device) if stats else None
+    d = _ffi.LayerNormDesc(x.data_ptr(), y.data_ptr(), _ptr(w), _ptr(b), _ptr(mean), _ptr(rstd), n, C, ld, 0, C, 0, dt, pdt, eps)
+    _ffi.check(_launch(x.device, lib.ydet_layer_norm, d), "ydet_layer_norm")
+    return y, mean, rstd
+
+
+def layer_norm_backward(dy, x, mean, rstd, weight=None, need=(True, True, True), bias_dtype=None):
+    """Gradients (dx, dweight, dbias) of layer_norm_forward from dy, its input and the statistics it returned.  `need` says
+    which of the three are wanted (the others are None); dweight has the weight's dtype, dbias `bias_dtype` (default: the
+    weight's; both fp32 without a weight).  Launches only: it can be captured into a graph."""
+    _need_cuda(dy, x, mean, rstd)
+    lib = _ffi.lib()
+    dt = _dt(x)
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError(f"dy is {dy.dtype} {tuple(dy.shape)}, x is {x.dtype} {tuple(x.shape)}")
+    if mean.shape != x.shape[:-1] or rstd.shape != x.shape[:-1] or mean.dtype != torch.float32 or rstd.dtype != torch.float32:
+        raise ValueError("mean and rstd are the fp32 tensors that layer_norm_forward returned for x")
+    dev = x.device
+    if not dev == dy.device == mean.device == rstd.device:
+        raise RuntimeError("layer_norm_backward: tensors on different devices")
+    x, n, ld = _as_rows(x, "layer_norm_backward")
+    dy, _, dy_ld = _as_rows(dy, "layer_norm_backward")
+    mean, rstd = mean.contiguous(), rstd.contiguous()
+    C = x.shape[-1]
+    (w,), pdt = _params(C, dev, weight)
+    wdt = torch.float32 if w is None else w.dtype
+    dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if need[0] else None
+    dw = torch.empty(C, device=dev, dtype=wdt) if need[1] else None
+    db = torch.empty(C, device=dev, dtype=wdt) if need[2] else None
+    nbytes = lib.ydet_layer_norm_backward_workspace_bytes(n, C) if need[1] or need[2] else 0
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+    d = _ffi.LayerNormGradDesc(dy.data_ptr(), x.data_ptr(), _ptr(dx), _ptr(w), mean.data_ptr(), rstd.data_ptr(), _ptr(dw), _ptr(db),
+                               n, C, dy_ld, 0, ld, 0, C, 0, dt, pdt)
+    _ffi.check(_launch(dev, lib.ydet_layer_norm_backward, d, _ptr(ws), nbytes), "ydet_layer_norm_backward")
+    if db is not None and bias_dtype is not None and db.dtype != bias_dtype:
+        db = db.to(bias_dtype)
+    return dx, dw, db
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = layer_norm_forward(x, weight, bias, eps)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        return layer_norm_backward(dy, x, mean, rstd, weight, need[:3], ctx.bias_dtype) + (None,)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """Layer normalisation over the last dimension, differentiable in x, weight and bias (once).  A recorded graph cannot be
+    captured (its leaves' gradients may belong to another stream): a captured training step calls layer_norm_forward and
+    layer_norm_backward."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        _need_cuda(x)
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("layer_norm: gradients are not recorded during graph capture; call layer_norm_forward and "
+                               "layer_norm_backward there")
+        return _LayerNorm.apply(x, weight, bias, eps)
+    return layer_norm_forward(x, weight, bias, eps, stats=False)[0]
+
+
+def _quantize(x, normalize, weight, bias, eps):
+    _need_cuda(x)
+    lib = _ffi.lib()
+    dt = _dt(x)
+    x, n, ld = _as_rows(x, "quantize_rows")
+    C = x.shape[-1]
+    (w, b), pdt = _params(C, x.device, weight, bias)
+    q_ld = (C + 15) // 16 * 16
+    q = torch.empty(x.shape[:-1] + (q_ld,), device=x.device, dtype=torch.int8)
+    scale = torch.empty(x.shape[:-1], device=x.device)
+    d = _ffi.QuantizeDesc(x.data_ptr(), q.data_ptr(), scale.data_ptr(), _ptr(w), _ptr(b), n, C, ld, 0, q_ld, dt, pdt, normalize, eps)
+    _ffi.check(_launch(x.device, lib.ydet_quantize_rows_i8, d), "ydet_quantize_rows_i8")
+    return (q if q_ld == C else q[..., :C]), scale
+
+
+@torch.no_grad()
+def quantize_rows(x):
+    """(q, scale): the rows of x [..., C] in 8 bits, q int8 of x's shape (its rows padded with zeros to 16 bytes in memory),
+    scale fp32 of x.shape[:-1] with x ~ q * scale.  scale = max|x| / 127; q is the integer nearest x / scale, ties to even.
+    A row with a NaN or an infinity has scale NaN and q = 0."""
+    return _quantize(x, 0, None, None, 0.0)
+
+
+@torch.no_grad()
+def layer_norm_quantize(x, weight=None, bias=None, eps=1e-5):
+    """quantize_rows(layer_norm(x, weight, bias, eps)) in one pass over x; the normalised values are not rounded in between."""
+    return _quantize(x, 1, weight, bias, eps)
+
+
+class LinearI8:
+    """Weights of a token-wise linear layer (or 1x1 convolution) in 8 bits, laid out for matmul_i8: wq int8 [N, K], one fp32
+    scale per output channel, an optional bias."""
+
+    def __init__(self, wq, scale, bias=None):
+        _need_cuda(wq, scale)
+        if wq.dim() != 2 or wq.dtype != torch.int8 or wq.numel() == 0:
+            raise ValueError(f"weights are int8 [N, K]: got {wq.dtype} {tuple(wq.shape)}")
+        self.N, self.K = wq.shape
+        dev = self.device = wq.device
+        for t in (scale, bias):
+            if t is not None and (t.shape != (self.N,) or t.device != dev or not t.is_floating_point()):
+                raise ValueError(f"scale and bias are floating [{self.N}] tensors on {dev}")
+        if self.K > 131071:
+            raise ValueError(f"K = {self.K}: 32-bit sums hold products of up to 131071 terms")
+        self.kp, self.n_pad = (self.K + 63) // 64 * 64, (self.N + 127) // 128 * 128
+        self.w = torch.zeros(self.n_pad, self.kp, device=dev, dtype=torch.int8)
+        self.w[:self.N, :self.K] = wq
+        self.scale = torch.zeros(self.n_pad, device=dev)
+        self.scale[:self.N] = scale.detach()
+        self.bias = None
+        if bias is not None:
+            self.bias = torch.zeros(self.n_pad, device=dev)
+            self.bias[:self.N] = bias.detach()
+
+    @classmethod
+    @torch.no_grad()
+    def quantize(cls, weight, bias=None):
+        """From floating weights [N, K] (or [N, K, 1, 1]): quantize_rows over every output channel's weights."""
+        if weight.dim() == 4 and weight.shape[2:] == (1, 1):
+            weight = weight[:, :, 0, 0]
+        if weight.dim() != 2:
+            raise ValueError(f"weights are [N, K] or [N, K, 1, 1]: got {tuple(weight.shape)}")
+        q, scale = quantize_rows(weight.detach())
+        return cls(q, scale, bias)
+
+
+_ACTS = {"none": _ffi.ACT_NONE, "leaky": _ffi.ACT_LEAKY, "silu": _ffi.ACT_SILU}
+_RES = {"after": _ffi.RES_AFTER_ACT, "before": _ffi.RES_BEFORE_ACT}
+
+
+@torch.no_grad()
+def matmul_i8(q, scale, lin, act="none", slope=0.1, res=None, res_mode="after", out_dtype=torch.bfloat16):
+    """act(q . lin.w^T * scale * lin.scale + lin.bias), [..., N] of out_dtype (bf16 or fp32), from int8 rows q [..., K] and
+    their scales [...] (quantize_rows).  act: "none", "leaky" (negative slope `slope`), "silu".  res [..., N] of out_dtype is
+    added after or before the activation (res_mode).  The sums are exact integers."""
+    _need_cuda(q, scale)
+    lib = _ffi.lib()
+    if act not in _ACTS or res_mode not in _RES:
+        raise ValueError(f"act {act!r} / res_mode {res_mode!r}: want one of {sorted(_ACTS)} / {sorted(_RES)}")
+    if q.dtype != torch.int8 or q.dim() == 0 or q.shape[-1] != lin.K:
+        raise ValueError(f"q is int8 [..., {lin.K}]: got {q.dtype} {tuple(q.shape)}")
+    dev, lead = q.device, q.shape[:-1]
+    if scale.shape != lead or scale.dtype != torch.float32:
+        raise ValueError(f"scale is fp32 {tuple(lead)}: got {scale.dtype} {tuple(scale.shape)}")
+    if out_dtype == torch.bfloat16:
+        odt = _ffi.BF16
+    elif out_dtype == torch.float32:
+        odt = _ffi.F32
+    else:
+        raise TypeError(f"unsupported dtype {out_dtype}")
+    if dev != lin.device or dev != scale.device or (res is not None and dev != res.device):
+        raise RuntimeError("matmul_i8: tensors on different devices")
+    q, n, ld = _as_rows(q, "matmul_i8")
+    if ld > 1 << 23:
+        q, ld = q.contiguous(), lin.K
+    # the library may read a row's last piece up to its 16-byte border: a view whose storage ends before that is copied
+    K16 = (lin.K + 15) // 16 * 16
+    if n and K16 != lin.K and ld % 16 == 0 and q.data_ptr() % 16 == 0 \
+            and q.storage_offset() + (n - 1) * ld + K16 > q.untyped_storage().nbytes():
+        q, ld = q.contiguous(), lin.K
+    scale = scale.contiguous()
+    rmode, rptr, r_ld = _ffi.RES_NONE, None, 0
+    if res is not None:
+        if res.shape != lead + (lin.N,) or res.dtype != out_dtype:
+            raise ValueError(f"res is {out_dtype} {tuple(lead) + (lin.N,)}: got {res.dtype} {tuple(res.shape)}")
+        res, _, r_ld = _as_rows(res.detach(), "matmul_i8")
+        rmode, rptr = _RES[res_mode], res.data_ptr()
+    y = torch.empty(lead + (lin.N,), device=dev, dtype=out_dtype)
+    d = _ffi.MatmulI8Desc(q.data_ptr(), scale.data_ptr(), lin.w.data_ptr(), lin.scale.data_ptr(), _ptr(lin.bias), rptr, y.data_ptr(),
+                          n, lin.K, lin.N, lin.kp, lin.n_pad, ld, 0, lin.N, 0, r_ld, 0, _ACTS[act], slope, rmode, odt)
+    _ffi.check(_launch(dev, lib.ydet_matmul_i8, d), "ydet_matmul_i8")
+    return y
+
+
+def linear_i8(x, lin, act="none", slope=0.1, res=None, res_mode="after", out_dtype=None):
+    """matmul_i8 of a floating map x [..., K], whose rows are quantised on the way; out_dtype defaults to x's."""
+    if x.shape[-1:] != (lin.K,):
+        raise ValueError(f"x is [..., {lin.K}]: got {tuple(x.shape)}")
+    q, scale = quantize_rows(x)
+    return matmul_i8(q, scale, lin, act, slope, res, res_mode, x.dtype if out_dtype is None else out_dtype)
