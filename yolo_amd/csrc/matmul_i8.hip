@@ -34,46 +34,93 @@ __device__ __forceinline__ i32x4 mma(const i32x4& a, const i32x4& b, const i32x4
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
 }
 
+// Epilogue variants, fixed at compile time so that a lane's values run through straight-line code: SiLU or leaky (slope 1 is "no
+// activation"), and where the residual goes in.
+template <bool SILU, int RES>
+struct Mode {
+    static constexpr bool silu = SILU;
+    static constexpr int res = RES;
+};
+template <typename F>
+__device__ __forceinline__ void with_mode(const Args& a, F f) {
+    if (a.act == YDET_ACT_SILU) {
+        if (a.res_mode == YDET_RES_NONE) f(Mode<true, YDET_RES_NONE>{});
+        else if (a.res_mode == YDET_RES_AFTER_ACT) f(Mode<true, YDET_RES_AFTER_ACT>{});
+        else f(Mode<true, YDET_RES_BEFORE_ACT>{});
+    } else {
+        if (a.res_mode == YDET_RES_NONE) f(Mode<false, YDET_RES_NONE>{});
+        else if (a.res_mode == YDET_RES_AFTER_ACT) f(Mode<false, YDET_RES_AFTER_ACT>{});
+        else f(Mode<false, YDET_RES_BEFORE_ACT>{});
+    }
+}
+template <typename M>
 __device__ __forceinline__ float finish(float v, float r, const Args& a) {
-    if (a.res_mode == YDET_RES_BEFORE_ACT) v += r;
-    v = conv::activate(v, a.act, a.slope);
-    return a.res_mode == YDET_RES_AFTER_ACT ? v + r : v;
+    if constexpr (M::res == YDET_RES_BEFORE_ACT) v += r;
+    if constexpr (M::silu) v = v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.44269504088896340736f));
+    else v = v > 0.f ? v : v * a.slope;
+    if constexpr (M::res == YDET_RES_AFTER_ACT) v += r;
+    return v;
 }
 
-// C consecutive channels n.. of pixel m: scales, bias, residual, activation, store.  C is 4, 8 or 16.
+// A run: C (4, 8 or 16) consecutive channels n.. of one pixel, in pieces of up to 16 bytes.
 template <typename OUT, int C>
-__device__ __forceinline__ void store_run(const Args& a, int m, int n, float xs, const int (&acc)[C]) {
-    constexpr int E = 16 / (int)sizeof(OUT);      // values of a 16-byte piece
-    typedef OUT piece __attribute__((ext_vector_type(E < C ? E : C)));
-    constexpr int PE = E < C ? E : C;
-    if (m >= a.M || n >= a.N) return;
-    float v[C];
+struct Run {
+    static constexpr int PE = 16 / (int)sizeof(OUT) < C ? 16 / (int)sizeof(OUT) : C, NP = C / PE;
+    typedef OUT piece __attribute__((ext_vector_type(PE)));
+    piece r[NP];        // the residual
+
+    template <typename M>
+    __device__ __forceinline__ void load_residual(const Args& a, int m, int n) {
+        if constexpr (M::res != YDET_RES_NONE) {
+            const OUT* p = reinterpret_cast<const OUT*>(a.res) + m * a.res_ld + n;
+#pragma unroll
+            for (int k = 0; k < NP; ++k) r[k] = piece{};
+            if (m >= a.M || n >= a.N) return;
+            if (a.vec) {
+#pragma unroll
+                for (int k = 0; k < NP; ++k) r[k] = *reinterpret_cast<const piece*>(p + k * PE);
+            } else {
+#pragma unroll
+                for (int i = 0; i < C; ++i)
+                    if (n + i < a.N) r[i / PE][i % PE] = p[i];
+            }
+        }
+    }
+    // ws, bias: the run's scales and biases
+    template <typename M>
+    __device__ __forceinline__ void store(const Args& a, int m, int n, float xs, const int (&acc)[C], const float (&ws)[C], const float (&bias)[C]) {
+        if (m >= a.M || n >= a.N) return;
+        OUT* y = reinterpret_cast<OUT*>(a.y) + m * a.y_ld + n;
+        piece o[NP];
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            float rr = 0.f;
+            if constexpr (M::res != YDET_RES_NONE) rr = (float)r[i / PE][i % PE];
+            o[i / PE][i % PE] = (OUT)finish<M>(fmaf((float)acc[i] * xs, ws[i], bias[i]), rr, a);
+        }
+        if (a.vec) {
+#pragma unroll
+            for (int k = 0; k < NP; ++k) *reinterpret_cast<piece*>(y + k * PE) = o[k];
+        } else {
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+                if (n + i < a.N) y[i] = o[i / PE][i % PE];
+        }
+    }
+};
+
+// scales and biases of C channels (both arrays are padded to n_pad values)
+template <int C>
+__device__ __forceinline__ void load_channels(const Args& a, int n, float (&ws)[C], float (&bias)[C]) {
 #pragma unroll
     for (int i = 0; i < C; i += 4) {
-        const float4 s = *reinterpret_cast<const float4*>(a.ws + n + i);
-        const float4 b = a.bias ? *reinterpret_cast<const float4*>(a.bias + n + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-        v[i] = fmaf((float)acc[i] * xs, s.x, b.x);
-        v[i + 1] = fmaf((float)acc[i + 1] * xs, s.y, b.y);
-        v[i + 2] = fmaf((float)acc[i + 2] * xs, s.z, b.z);
-        v[i + 3] = fmaf((float)acc[i + 3] * xs, s.w, b.w);
-    }
-    OUT* y = reinterpret_cast<OUT*>(a.y) + m * a.y_ld + n;
-    const OUT* res = a.res_mode == YDET_RES_NONE ? nullptr : reinterpret_cast<const OUT*>(a.res) + m * a.res_ld + n;
-    if (a.vec) {
-        piece r[C / PE];
-#pragma unroll
-        for (int p = 0; p < C / PE; ++p) r[p] = res ? *reinterpret_cast<const piece*>(res + p * PE) : piece{};
-#pragma unroll
-        for (int p = 0; p < C / PE; ++p) {
-            piece o;
-#pragma unroll
-            for (int e = 0; e < PE; ++e) o[e] = (OUT)finish(v[p * PE + e], (float)r[p][e], a);
-            *reinterpret_cast<piece*>(y + p * PE) = o;
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f), b = s;
+        if (n + i < a.n_pad) {
+            s = *reinterpret_cast<const float4*>(a.ws + n + i);
+            if (a.bias) b = *reinterpret_cast<const float4*>(a.bias + n + i);
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < C; ++i)
-            if (n + i < a.N) y[i] = (OUT)finish(v[i], res ? (float)res[i] : 0.f, a);
+        ws[i] = s.x, ws[i + 1] = s.y, ws[i + 2] = s.z, ws[i + 3] = s.w;
+        bias[i] = b.x, bias[i + 1] = b.y, bias[i + 2] = b.z, bias[i + 3] = b.w;
     }
 }
 
@@ -204,21 +251,31 @@ __global__ __launch_bounds__(64 * WAVES_N * WAVES_M, 2) void tile_kernel(const A
     else stage_step(N, N, Y, kt);
 
     // lane (q, p): pixel p of every pixel fragment, channels 16 q .. + 15 of every 64-channel group
-    const int q = lane >> 4, p = lane & 15;
+    const int q = lane >> 4, p = lane & 15, mw = m0 + wm * WM + p;
+    float xs[FM];
 #pragma unroll
-    for (int j = 0; j < FM; ++j) {
-        const int m = m0 + wm * WM + j * 16 + p;
-        const float xs = m < a.M ? a.xs[m] : 0.f;
+    for (int j = 0; j < FM; ++j) xs[j] = mw + j * 16 < a.M ? a.xs[mw + j * 16] : 0.f;
+    with_mode(a, [&](auto mode) {
+        using M = decltype(mode);
 #pragma unroll
-        for (int gI = 0; gI < FN / 4; ++gI) {
-            int v[16];
+        for (int g = 0; g < FN / 4; ++g) {
+            const int n = n0 + wn * WN + g * 64 + q * 16;
+            float ws[16], bias[16];
+            load_channels<16>(a, n, ws, bias);
+            Run<OUT, 16> run[FM];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int j = 0; j < FM; ++j) run[j].template load_residual<M>(a, mw + j * 16, n);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[i * 4 + e] = acc[gI * 4 + i][j][e];
-            store_run<OUT, 16>(a, m, n0 + wn * WN + gI * 64 + q * 16, xs, v);
+            for (int j = 0; j < FM; ++j) {
+                int v[16];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[i * 4 + e] = acc[g * 4 + i][j][e];
+                run[j].template store<M>(a, mw + j * 16, n, xs[j], v, ws, bias);
+            }
         }
-    }
+    });
 }
 
 // ---- few rows: the K of a small tile is shared by the waves of a workgroup ------------------------------------------------
@@ -300,19 +357,27 @@ __global__ __launch_bounds__(64 * NW) void few_rows_kernel(const Args a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[i * 4 + e] = s[e];
         }
-        const int m = m0 + j * 16 + p;
-        store_run<OUT, 4 * FN>(a, m, n0 + q * 4 * FN, m < a.M ? a.xs[m] : 0.f, v);
+        const int m = m0 + j * 16 + p, n = n0 + q * 4 * FN;
+        float ws[4 * FN], bias[4 * FN];
+        load_channels<4 * FN>(a, n, ws, bias);
+        with_mode(a, [&](auto mode) {
+            using M = decltype(mode);
+            Run<OUT, 4 * FN> run;
+            run.template load_residual<M>(a, m, n);
+            run.template store<M>(a, m, n, m < a.M ? a.xs[m] : 0.f, v, ws, bias);
+        });
     }
 }
 
 template <typename OUT, int BN, int BM, int WAVES_N, int WAVES_M>
 static int launch_tile(Args a, hipStream_t stream) {
-    constexpr int lds = 2 * (BN + BM) * 128;
+    constexpr int most = 2 * (BN + BM) * 128;
+    const int lds = a.kp <= 128 ? most / 2 : most;      // (a single stage leaves room for twice the workgroups)
     a.tiles_n = (a.N + BN - 1) / BN;
     const long long blocks = (long long)a.tiles_n * ((a.M + BM - 1) / BM);
     YDET_CHECK_ARG(blocks * 64 * WAVES_N * WAVES_M <= UINT32_MAX, "matmul_i8: %d rows x %d channels are too many tiles", a.M, a.N);
     static unsigned char done[kMaxDevices];
-    const int rc = raise_dynamic_lds_limit(reinterpret_cast<const void*>(&tile_kernel<OUT, BN, BM, WAVES_N, WAVES_M>), lds, done, "matmul_i8");
+    const int rc = raise_dynamic_lds_limit(reinterpret_cast<const void*>(&tile_kernel<OUT, BN, BM, WAVES_N, WAVES_M>), most, done, "matmul_i8");
     if (rc != YDET_OK) return rc;
     hipLaunchKernelGGL((tile_kernel<OUT, BN, BM, WAVES_N, WAVES_M>), dim3((unsigned)blocks), dim3(64 * WAVES_N * WAVES_M), lds, stream, a);
     YDET_CHECK_LAUNCH("matmul_i8");
@@ -369,7 +434,7 @@ int ydet_launch_matmul_i8(const ydet_matmul_i8_desc* d, hipStream_t stream) {
     if (a.res_mode != YDET_RES_NONE) a.res = static_cast<const char*>(d->res) + d->res_coff * es;
     YDET_CHECK_ARG(((uintptr_t)a.y | (uintptr_t)a.res) % es == 0 && (uintptr_t)a.xs % 4 == 0, "matmul_i8: misaligned tensor");
     a.M = (int)d->rows, a.K = d->K, a.N = d->N, a.kp = d->kp, a.n_pad = d->n_pad;
-    a.x_ld = d->x_ld, a.y_ld = d->y_ld, a.res_ld = d->res_ld, a.act = d->act, a.slope = d->slope;
+    a.x_ld = d->x_ld, a.y_ld = d->y_ld, a.res_ld = d->res_ld, a.act = d->act, a.slope = d->act == YDET_ACT_LEAKY ? d->slope : 1.f;
     auto wide = [&](const char* p, int ld) { return (uintptr_t)p % 16 == 0 && ld * es % 16 == 0; };
     a.vec = d->N % 16 == 0 && wide(a.y, d->y_ld) && (a.res_mode == YDET_RES_NONE || wide(a.res, d->res_ld));
     // rows read in 16-byte pieces: the last piece of a row may reach behind K, so the pitch has to hold it

@@ -290,9 +290,9 @@ MAX_ROW = 8192      # channels of a row that layer_norm and quantize_rows take
 def _launch(dev, call, *args):
     """`call(*args, stream)` on torch's current stream of `dev`."""
     if torch.cuda.current_device() == dev.index:
-        return call(*args, torch.cuda.current_stream().cuda_stream)
+        return call(*args, torch._C._cuda_getCurrentRawStream(dev.index))
     with torch.cuda.device(dev):
-        return call(*args, torch.cuda.current_stream().cuda_stream)
+        return call(*args, torch._C._cuda_getCurrentRawStream(dev.index))
 
 
 def _as_rows(t, what):
@@ -313,41 +313,78 @@ def _as_rows(t, what):
     return t.contiguous(), n, C
 
 
-def _params(C, dev, *ps):
+def _params(C, dev, w, b):
     """The per-channel parameters (None allowed) as contiguous tensors of one type, and that type."""
-    dts = set()
-    for p in ps:
-        if p is None:
-            continue
-        if p.shape != (C,):
-            raise ValueError(f"weight and bias have one value a channel: got {tuple(p.shape)} for {C} channels")
-        if p.device != dev:
-            raise RuntimeError(f"weight / bias on {p.device}, the input on {dev}")
-        dts.add(_dt(p))
-    dt = _ffi.F32 if len(dts) != 1 else dts.pop()
+    dt = None
+    for p in (w, b):
+        if p is not None:
+            if p.dim() != 1 or p.shape[0] != C:
+                raise ValueError(f"weight and bias have one value a channel: got {tuple(p.shape)} for {C} channels")
+            if p.device != dev:
+                raise RuntimeError(f"weight / bias on {p.device}, the input on {dev}")
+            d = _dt(p)
+            dt = d if dt is None or dt == d else _ffi.F32
+    dt = _ffi.F32 if dt is None else dt
     td = torch.float32 if dt == _ffi.F32 else torch.bfloat16
-    return [p if p is None else p.detach().to(td).contiguous() for p in ps], dt
+    if w is not None and (w.dtype != td or not w.is_contiguous()):
+        w = w.detach().to(td).contiguous()
+    if b is not None and (b.dtype != td or not b.is_contiguous()):
+        b = b.detach().to(td).contiguous()
+    return w, b, dt
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, stats=True):
-    """Layer normalisation over the last dimension: (y, mean, rstd), y of x's dtype and shape, mean and rstd fp32 of
-    x.shape[:-1] (None without `stats`).  weight, bias: [C] fp32 or bf16, or None."""
+def _ln_forward(x, weight, bias, eps, stats):
+    """(y, statistics): the means of all rows and then their reciprocal deviations in one fp32 buffer, or None."""
     _need_cuda(x)
-    lib = _ffi.lib()
     dt = _dt(x)
     x, n, ld = _as_rows(x, "layer_norm")
-    C = x.shape[-1]
-    (w, b), pdt = _params(C, x.device, weight, bias)
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    mean = torch.empty(x.shape[:-1], device=x.device) if stats else None
-    rstd = torch.empty(x.shape[:-1], device=x.device) if stats else None
-    d = _ffi.LayerNormDesc(x.data_ptr(), y.data_ptr(), _ptr(w), _ptr(b), _ptr(mean), _ptr(rstd), n, C, ld, 0, C, 0, dt, pdt, eps)
-    _ffi.check(_launch(x.device, lib.ydet_layer_norm, d), "ydet_layer_norm")
-    return y, mean, rstd
+    C, dev = x.shape[-1], x.device
+    w, b, pdt = _params(C, dev, weight, bias)
+    y = torch.empty(x.shape, device=dev, dtype=x.dtype)
+    st = torch.empty((2,) + x.shape[:-1], device=dev, dtype=torch.float32) if stats else None
+    mean = st.data_ptr() if stats else None
+    d = _ffi.LayerNormDesc(x.data_ptr(), y.data_ptr(), _ptr(w), _ptr(b), mean, mean and mean + 4 * n, n, C, ld, 0, C, 0, dt, pdt, eps)
+    rc = _launch(dev, _ffi.lib().ydet_layer_norm, d)
+    if rc:
+        _ffi.check(rc, "ydet_layer_norm")
+    return y, st
+
+
+def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
+    """Layer normalisation over the last dimension: (y, mean, rstd), y of x's dtype and shape, mean and rstd fp32 of
+    x.shape[:-1].  weight, bias: [C] fp32 or bf16, or None."""
+    y, st = _ln_forward(x, weight, bias, eps, True)
+    return y, st[0], st[1]
+
+
+def _ln_backward(dy, x, mean, rstd, weight, need, bias_dtype):
+    """mean, rstd: addresses."""
+    lib = _ffi.lib()
+    dt = _dt(x)
+    x, n, ld = _as_rows(x, "layer_norm_backward")
+    dy, _, dy_ld = _as_rows(dy, "layer_norm_backward")
+    C, dev = x.shape[-1], x.device
+    w, _, pdt = _params(C, dev, weight, None)
+    wdt = torch.float32 if w is None else w.dtype
+    dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if need[0] else None
+    dw = torch.empty(C, device=dev, dtype=wdt) if need[1] else None
+    db = torch.empty(C, device=dev, dtype=wdt) if need[2] else None
+    ws, nbytes = None, 0
+    if need[1] or need[2]:
+        nbytes = lib.ydet_layer_norm_backward_workspace_bytes(n, C)
+        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    d = _ffi.LayerNormGradDesc(dy.data_ptr(), x.data_ptr(), _ptr(dx), _ptr(w), mean, rstd, _ptr(dw), _ptr(db),
+                               n, C, dy_ld, 0, ld, 0, C, 0, dt, pdt)
+    rc = _launch(dev, lib.ydet_layer_norm_backward, d, _ptr(ws), nbytes)
+    if rc:
+        _ffi.check(rc, "ydet_layer_norm_backward")
+    if db is not None and bias_dtype is not None and bias_dtype != wdt:
+        db = db.to(bias_dtype)
+    return dx, dw, db
 
 
 def layer_norm_backward(dy, x, mean, rstd, weight=None, need=(True, True, True), bias_dtype=None):
@@ -355,48 +392,35 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, need=(True, True, True),
     which of the three are wanted (the others are None); dweight has the weight's dtype, dbias `bias_dtype` (default: the
     weight's; both fp32 without a weight).  Launches only: it can be captured into a graph."""
     _need_cuda(dy, x, mean, rstd)
-    lib = _ffi.lib()
-    dt = _dt(x)
     if dy.shape != x.shape or dy.dtype != x.dtype:
         raise ValueError(f"dy is {dy.dtype} {tuple(dy.shape)}, x is {x.dtype} {tuple(x.shape)}")
     if mean.shape != x.shape[:-1] or rstd.shape != x.shape[:-1] or mean.dtype != torch.float32 or rstd.dtype != torch.float32:
         raise ValueError("mean and rstd are the fp32 tensors that layer_norm_forward returned for x")
-    dev = x.device
-    if not dev == dy.device == mean.device == rstd.device:
+    if not x.device == dy.device == mean.device == rstd.device:
         raise RuntimeError("layer_norm_backward: tensors on different devices")
-    x, n, ld = _as_rows(x, "layer_norm_backward")
-    dy, _, dy_ld = _as_rows(dy, "layer_norm_backward")
     mean, rstd = mean.contiguous(), rstd.contiguous()
-    C = x.shape[-1]
-    (w,), pdt = _params(C, dev, weight)
-    wdt = torch.float32 if w is None else w.dtype
-    dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if need[0] else None
-    dw = torch.empty(C, device=dev, dtype=wdt) if need[1] else None
-    db = torch.empty(C, device=dev, dtype=wdt) if need[2] else None
-    nbytes = lib.ydet_layer_norm_backward_workspace_bytes(n, C) if need[1] or need[2] else 0
-    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
-    d = _ffi.LayerNormGradDesc(dy.data_ptr(), x.data_ptr(), _ptr(dx), _ptr(w), mean.data_ptr(), rstd.data_ptr(), _ptr(dw), _ptr(db),
-                               n, C, dy_ld, 0, ld, 0, C, 0, dt, pdt)
-    _ffi.check(_launch(dev, lib.ydet_layer_norm_backward, d, _ptr(ws), nbytes), "ydet_layer_norm_backward")
-    if db is not None and bias_dtype is not None and db.dtype != bias_dtype:
-        db = db.to(bias_dtype)
-    return dx, dw, db
+    return _ln_backward(dy, x, mean.data_ptr(), rstd.data_ptr(), weight, need, bias_dtype)
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = layer_norm_forward(x, weight, bias, eps)
-        ctx.save_for_backward(x, weight, mean, rstd)
+        y, st = _ln_forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, st)
         ctx.bias_dtype = None if bias is None else bias.dtype
         return y
 
+    def _gradients(ctx, dy):
+        x, weight, st = ctx.saved_tensors
+        mean = st.data_ptr()
+        return _ln_backward(dy, x, mean, mean + 2 * st.numel(), weight, ctx.needs_input_grad, ctx.bias_dtype) + (None,)
+
+    _gradients_once = torch.autograd.function.once_differentiable(_gradients)
+
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        return layer_norm_backward(dy, x, mean, rstd, weight, need[:3], ctx.bias_dtype) + (None,)
+        # (grad mode is on here only where a second derivative was asked for: its use is an error)
+        return _LayerNorm._gradients_once(ctx, dy) if torch.is_grad_enabled() else _LayerNorm._gradients(ctx, dy)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -409,25 +433,25 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
             raise RuntimeError("layer_norm: gradients are not recorded during graph capture; call layer_norm_forward and "
                                "layer_norm_backward there")
         return _LayerNorm.apply(x, weight, bias, eps)
-    return layer_norm_forward(x, weight, bias, eps, stats=False)[0]
+    return _ln_forward(x, weight, bias, eps, False)[0]
 
 
 def _quantize(x, normalize, weight, bias, eps):
     _need_cuda(x)
-    lib = _ffi.lib()
     dt = _dt(x)
     x, n, ld = _as_rows(x, "quantize_rows")
-    C = x.shape[-1]
-    (w, b), pdt = _params(C, x.device, weight, bias)
+    C, dev, lead = x.shape[-1], x.device, x.shape[:-1]
+    w, b, pdt = _params(C, dev, weight, bias)
     q_ld = (C + 15) // 16 * 16
-    q = torch.empty(x.shape[:-1] + (q_ld,), device=x.device, dtype=torch.int8)
-    scale = torch.empty(x.shape[:-1], device=x.device)
+    q = torch.empty(lead + (q_ld,), device=dev, dtype=torch.int8)
+    scale = torch.empty(lead, device=dev, dtype=torch.float32)
     d = _ffi.QuantizeDesc(x.data_ptr(), q.data_ptr(), scale.data_ptr(), _ptr(w), _ptr(b), n, C, ld, 0, q_ld, dt, pdt, normalize, eps)
-    _ffi.check(_launch(x.device, lib.ydet_quantize_rows_i8, d), "ydet_quantize_rows_i8")
+    rc = _launch(dev, _ffi.lib().ydet_quantize_rows_i8, d)
+    if rc:
+        _ffi.check(rc, "ydet_quantize_rows_i8")
     return (q if q_ld == C else q[..., :C]), scale
 
 
-@torch.no_grad()
 def quantize_rows(x):
     """(q, scale): the rows of x [..., C] in 8 bits, q int8 of x's shape (its rows padded with zeros to 16 bytes in memory),
     scale fp32 of x.shape[:-1] with x ~ q * scale.  scale = max|x| / 127; q is the integer nearest x / scale, ties to even.
@@ -435,7 +459,6 @@ def quantize_rows(x):
     return _quantize(x, 0, None, None, 0.0)
 
 
-@torch.no_grad()
 def layer_norm_quantize(x, weight=None, bias=None, eps=1e-5):
     """quantize_rows(layer_norm(x, weight, bias, eps)) in one pass over x; the normalised values are not rounded in between."""
     return _quantize(x, 1, weight, bias, eps)
@@ -482,7 +505,6 @@ _ACTS = {"none": _ffi.ACT_NONE, "leaky": _ffi.ACT_LEAKY, "silu": _ffi.ACT_SILU}
 _RES = {"after": _ffi.RES_AFTER_ACT, "before": _ffi.RES_BEFORE_ACT}
 
 
-@torch.no_grad()
 def matmul_i8(q, scale, lin, act="none", slope=0.1, res=None, res_mode="after", out_dtype=torch.bfloat16):
     """act(q . lin.w^T * scale * lin.scale + lin.bias), [..., N] of out_dtype (bf16 or fp32), from int8 rows q [..., K] and
     their scales [...] (quantize_rows).  act: "none", "leaky" (negative slope `slope`), "silu".  res [..., N] of out_dtype is
@@ -522,7 +544,9 @@ def matmul_i8(q, scale, lin, act="none", slope=0.1, res=None, res_mode="after", 
     y = torch.empty(lead + (lin.N,), device=dev, dtype=out_dtype)
     d = _ffi.MatmulI8Desc(q.data_ptr(), scale.data_ptr(), lin.w.data_ptr(), lin.scale.data_ptr(), _ptr(lin.bias), rptr, y.data_ptr(),
                           n, lin.K, lin.N, lin.kp, lin.n_pad, ld, 0, lin.N, 0, r_ld, 0, _ACTS[act], slope, rmode, odt)
-    _ffi.check(_launch(dev, lib.ydet_matmul_i8, d), "ydet_matmul_i8")
+    rc = _launch(dev, lib.ydet_matmul_i8, d)
+    if rc:
+        _ffi.check(rc, "ydet_matmul_i8")
     return y
 
 
