@@ -546,6 +546,13 @@ typedef struct {
 } ydet_matmul_i8_desc;
 int ydet_matmul_i8(const ydet_matmul_i8_desc* d, void* stream);
 
+/* ydet_quantize_rows_i8 and ydet_matmul_i8 behind each other, the 8-bit rows in the caller's workspace
+ * (ydet_linear_i8_workspace_bytes(rows, K), 16-byte aligned): `in` without q, scale and q_ld, `product` without x, x_scale, x_ld
+ * and x_coff; in->rows == product->rows, in->C == product->K. */
+size_t ydet_linear_i8_workspace_bytes(int64_t rows, int K);
+int ydet_linear_i8(const ydet_quantize_desc* in, const ydet_matmul_i8_desc* product, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
 /* ------------------------------------------------------------------------------------------
  * Launch-list executor: one call runs a whole pre-planned forward pass
  * (the Python loop of Model.forward_once, yolov5_official/model.py:220-234, and the forward()

@@ -62,10 +62,19 @@ __device__ __forceinline__ float finish(float v, float r, const Args& a) {
     return v;
 }
 
-// A run: C (4, 8 or 16) consecutive channels n.. of one pixel, in pieces of up to 16 bytes.
-template <typename OUT, int C>
+// Which channel of a group of 16 F (F fragments: F MFMA row blocks of 16) MFMA row (q, e) of fragment i holds.  A lane ends with the
+// rows 4 q .. 4 q + 3 of every fragment; in this order they are pieces of PE consecutive channels (16 bytes of output), and the
+// four lane groups' pieces lie side by side: one store writes 64 consecutive bytes of each of 16 pixels.
+template <int PE>
+__device__ __forceinline__ int channel_of(int i, int q, int e) {
+    return PE == 8 ? (i >> 1) * 32 + q * 8 + (i & 1) * 4 + e : i * 16 + q * 4 + e;
+}
+
+// What a lane holds of one pixel in a group of 16 F channels: NP pieces of PE channels, piece k from channel n + 4 PE k on
+// (n: the group's first channel + PE q).
+template <typename OUT, int F>
 struct Run {
-    static constexpr int PE = 16 / (int)sizeof(OUT) < C ? 16 / (int)sizeof(OUT) : C, NP = C / PE;
+    static constexpr int PE = F == 1 ? 4 : 16 / (int)sizeof(OUT), NP = 4 * F / PE, C = 4 * F;
     typedef OUT piece __attribute__((ext_vector_type(PE)));
     piece r[NP];        // the residual
 
@@ -74,67 +83,73 @@ struct Run {
         if constexpr (M::res != YDET_RES_NONE) {
             const OUT* p = reinterpret_cast<const OUT*>(a.res) + m * a.res_ld + n;
 #pragma unroll
-            for (int k = 0; k < NP; ++k) r[k] = piece{};
-            if (m >= a.M || n >= a.N) return;
-            if (a.vec) {
+            for (int k = 0; k < NP; ++k) {
+                r[k] = piece{};
+                if (m < a.M && n + 4 * PE * k < a.N) {
+                    if (a.vec) {
+                        r[k] = *reinterpret_cast<const piece*>(p + 4 * PE * k);
+                    } else {
 #pragma unroll
-                for (int k = 0; k < NP; ++k) r[k] = *reinterpret_cast<const piece*>(p + k * PE);
-            } else {
-#pragma unroll
-                for (int i = 0; i < C; ++i)
-                    if (n + i < a.N) r[i / PE][i % PE] = p[i];
+                        for (int e = 0; e < PE; ++e)
+                            if (n + 4 * PE * k + e < a.N) r[k][e] = p[4 * PE * k + e];
+                    }
+                }
             }
         }
     }
-    // ws, bias: the run's scales and biases
+    // acc: the pieces' sums; ws, bias: their channels' scales and biases
     template <typename M>
     __device__ __forceinline__ void store(const Args& a, int m, int n, float xs, const int (&acc)[C], const float (&ws)[C], const float (&bias)[C]) {
-        if (m >= a.M || n >= a.N) return;
+        if (m >= a.M) return;
         OUT* y = reinterpret_cast<OUT*>(a.y) + m * a.y_ld + n;
-        piece o[NP];
 #pragma unroll
-        for (int i = 0; i < C; ++i) {
-            float rr = 0.f;
-            if constexpr (M::res != YDET_RES_NONE) rr = (float)r[i / PE][i % PE];
-            o[i / PE][i % PE] = (OUT)finish<M>(fmaf((float)acc[i] * xs, ws[i], bias[i]), rr, a);
-        }
-        if (a.vec) {
+        for (int k = 0; k < NP; ++k) {
+            piece o;
 #pragma unroll
-            for (int k = 0; k < NP; ++k) *reinterpret_cast<piece*>(y + k * PE) = o[k];
-        } else {
+            for (int e = 0; e < PE; ++e) {
+                float rr = 0.f;
+                if constexpr (M::res != YDET_RES_NONE) rr = (float)r[k][e];
+                o[e] = (OUT)finish<M>(fmaf((float)acc[k * PE + e] * xs, ws[k * PE + e], bias[k * PE + e]), rr, a);
+            }
+            if (a.vec) {
+                if (n + 4 * PE * k < a.N) *reinterpret_cast<piece*>(y + 4 * PE * k) = o;
+            } else {
 #pragma unroll
-            for (int i = 0; i < C; ++i)
-                if (n + i < a.N) y[i] = o[i / PE][i % PE];
+                for (int e = 0; e < PE; ++e)
+                    if (n + 4 * PE * k + e < a.N) y[4 * PE * k + e] = o[e];
+            }
         }
     }
 };
 
-// scales and biases of C channels (both arrays are padded to n_pad values)
-template <int C>
-__device__ __forceinline__ void load_channels(const Args& a, int n, float (&ws)[C], float (&bias)[C]) {
+// scales and biases of a run's channels, from memory or LDS (both arrays are padded to whole groups)
+template <typename R>
+__device__ __forceinline__ void load_channels(const float* ws, const float* bias, float (&s)[R::C], float (&b)[R::C]) {
 #pragma unroll
-    for (int i = 0; i < C; i += 4) {
-        float4 s = make_float4(0.f, 0.f, 0.f, 0.f), b = s;
-        if (n + i < a.n_pad) {
-            s = *reinterpret_cast<const float4*>(a.ws + n + i);
-            if (a.bias) b = *reinterpret_cast<const float4*>(a.bias + n + i);
+    for (int k = 0; k < R::NP; ++k)
+#pragma unroll
+        for (int e = 0; e < R::PE; ++e) {
+            s[k * R::PE + e] = ws[4 * R::PE * k + e];
+            b[k * R::PE + e] = bias ? bias[4 * R::PE * k + e] : 0.f;
         }
-        ws[i] = s.x, ws[i + 1] = s.y, ws[i + 2] = s.z, ws[i + 3] = s.w;
-        bias[i] = b.x, bias[i + 1] = b.y, bias[i + 2] = b.z, bias[i + 3] = b.w;
-    }
 }
 
 // ---- tiles: BN channels x BM pixels, operands through LDS --------------------------------------------------------------
 // LDS image of a stage: BN weight rows, then BM pixel rows, 128 bytes of K each; row r's 16-byte piece c lies at place
 // c ^ ((r >> 1) & 7), so that the 16 rows a fragment read touches fall into 16 different places of the banks.  Stages are filled by
 // LDS-DMA (eight rows an instruction); rows behind the last pixel and channels behind n_pad lie outside the buffer
-// descriptors and read as zeros.  Two stages; the fragments of a half stage are read while the previous half's MFMAs run.
-template <typename OUT, int BN, int BM, int WAVES_N, int WAVES_M>
+// descriptors and read as zeros.  NST stages; the fragments of a half stage are read while the previous half's MFMAs run.
+// What bounds it: for long K the operands' way through L2 (52 us for 23104 x 4096 -> 512 with 256 x 192 tiles: 1.85 POP/s, where a
+// library product of 8192^3 reaches 2.06), for short K the rows and the output (52 us for 409600 x 128 -> 128 with SiLU and
+// residual: 5.0 TB/s), for many channels and short K the epilogue, about ten operations a value, two of them transcendental
+// (70 us for 102400 x 256 -> 1024, half of which the vector units are busy).
+template <typename OUT, int BN, int BM, int WAVES_N, int WAVES_M, int NST = 2>
 __global__ __launch_bounds__(64 * WAVES_N * WAVES_M, 2) void tile_kernel(const Args a) {
     constexpr int NW = WAVES_N * WAVES_M, WN = BN / WAVES_N, WM = BM / WAVES_M, FN = WN / 16, FM = WM / 16;
     constexpr int RB = 128, STAGE = (BN + BM) * RB, LW = BN / 8 / NW, LX = BM / 8 / NW;
     static_assert(WN % 64 == 0 && BN % (8 * NW) == 0 && BM % (8 * NW) == 0, "tile shape");
     extern __shared__ __attribute__((aligned(128))) char smem[];
+    char* const stages = smem + (2 * BN + BM) * 4;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wn = wave % WAVES_N, wm = wave / WAVES_N;
     const unsigned t = xcd_remap(blockIdx.x, gridDim.x);
@@ -146,12 +161,12 @@ __global__ __launch_bounds__(64 * WAVES_N * WAVES_M, 2) void tile_kernel(const A
                                                                         (int)(w_span < cap ? (unsigned)w_span : cap), 0x00020000);
     const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(a.x + m0 * a.x_ld), 0,
                                                                         (int)(x_span < cap ? (unsigned)x_span : cap), 0x00020000);
+    const int halves = a.kp / 64, nk = (halves + 1) / 2;
     unsigned ow[LW], ox[LX];
 #pragma unroll
     for (int j = 0; j < LW; ++j) {
         const int r = (j * NW + wave) * 8 + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
-        // LDS row (i, q, e) of a 64-channel group holds channel (q, i, e): fragment i, lane group q, register e
-        const int chan = (r & ~63) + ((r >> 2) & 3) * 16 + ((r >> 4) & 3) * 4 + (r & 3);
+        const int chan = (r & ~63) + channel_of<Run<OUT, 4>::PE>((r >> 4) & 3, (r >> 2) & 3, r & 3);
         ow[j] = (unsigned)chan * (unsigned)a.kp + c * 16;
     }
 #pragma unroll
@@ -159,24 +174,42 @@ __global__ __launch_bounds__(64 * WAVES_N * WAVES_M, 2) void tile_kernel(const A
         const int r = (j * NW + wave) * 8 + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
         ox[j] = (unsigned)r * (unsigned)a.x_ld + c * 16;
     }
+    // scales of the tile's channels and rows, and the biases, wait in LDS in front of the stages: the epilogue reads memory for
+    // the residual only
+    float* sc = reinterpret_cast<float*>(smem);         // [BN] channel scales, [BN] biases, [BM] row scales
+    {
+        const float* none = nullptr;
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.ws + n0), 0, (a.n_pad - n0) * 4, 0x00020000);
+        const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.bias ? a.bias + n0 : none), 0,
+                                                                            a.bias ? (a.n_pad - n0) * 4 : 0, 0x00020000);
+        const __amdgpu_buffer_rsrc_t rr = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.xs + m0), 0, (BM < a.M - m0 ? BM : a.M - m0) * 4,
+                                                                            0x00020000);
+        for (int k = wave; k < (2 * BN + BM) / 64; k += NW) {
+            __attribute__((address_space(3))) void* dst = (__attribute__((address_space(3))) void*)(sc + k * 64);
+            if (k < BN / 64) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, dst, 4, lane * 4, k * 256, 0, 0);
+            else if (k < 2 * BN / 64) __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, dst, 4, lane * 4, (k - BN / 64) * 256, 0, 0);
+            else __builtin_amdgcn_raw_ptr_buffer_load_lds(rr, dst, 4, lane * 4, (k - 2 * BN / 64) * 256, 0, 0);
+        }
+    }
     auto issue = [&](int stage, int kt) {
-        char* dst = smem + stage * STAGE + wave * 1024;
+        kt *= RB;
+        char* dst = stages + stage * STAGE + wave * 1024;
 #pragma unroll
         for (int j = 0; j < LW; ++j)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (__attribute__((address_space(3))) void*)(dst + j * NW * 1024), 16, (int)ow[j],
-                                                     kt * RB, 0, 0);
+                                                     kt, 0, 0);
 #pragma unroll
         for (int j = 0; j < LX; ++j)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (__attribute__((address_space(3))) void*)(dst + BN * RB + j * NW * 1024), 16,
-                                                     (int)ox[j], kt * RB, 0, 0);
+                                                     (int)ox[j], kt, 0, 0);
     };
     int fo[2];
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) fo[kk] = (lane & 15) * RB + (((kk * 4 + (lane >> 4)) ^ ((lane & 15) >> 1)) * 16);
     i32x4 fa[2][FN], fb[2][FM], acc[FN][FM];
     auto read = [&](int stage, int kk, i32x4 (&A)[FN], i32x4 (&B)[FM]) {
-        const char* pw = smem + stage * STAGE + wn * WN * RB + fo[kk];
-        const char* px = smem + stage * STAGE + (BN + wm * WM) * RB + fo[kk];
+        const char* pw = stages + stage * STAGE + wn * WN * RB + fo[kk];
+        const char* px = stages + stage * STAGE + (BN + wm * WM) * RB + fo[kk];
 #pragma unroll
         for (int i = 0; i < FN; ++i) A[i] = *reinterpret_cast<const i32x4*>(pw + i * 16 * RB);
 #pragma unroll
@@ -193,24 +226,23 @@ __global__ __launch_bounds__(64 * WAVES_N * WAVES_M, 2) void tile_kernel(const A
 #pragma unroll
         for (int j = 0; j < FM; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
 
-    const int halves = a.kp / 64, nk = (halves + 1) / 2;
-    issue(0, 0);
-    if (nk > 1) {
-        issue(1, 1);
-        conv::wait_vmcnt<LW + LX>();
-    } else {
-        conv::wait_vmcnt<0>();
-    }
+    constexpr int L = LW + LX;
+#pragma unroll
+    for (int k = 0; k < NST; ++k)
+        if (k < nk) issue(k, k);
+    if (nk >= NST) conv::wait_vmcnt<(NST - 1) * L>();       // (the scales are older than every stage)
+    else conv::wait_vmcnt<0>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     read(0, 0, fa[0], fb[0]);
     // One stage: its second half is read under the first half's MFMAs; then every wave has its fragments and its own pieces
     // of the next stage, the barrier makes both common, the stage is refilled and the next one's first half is read under the second
-    // half's MFMAs.  REFILL / MORE / WHOLE: a stage after the next, a next stage, a second half exist (compile-time, so
+    // half's MFMAs.  REFILL / MORE / WHOLE: a stage to refill, a next stage, a second half exist (compile-time, so
     // that reads and MFMAs share a basic block).
+    int cur = 0;
     auto stage_step = [&](auto refill, auto more, auto whole, int kt) {
         constexpr bool REFILL = decltype(refill)::value, MORE = decltype(more)::value, WHOLE = decltype(whole)::value;
-        const int cur = kt & 1;
+        const int next = cur + 1 == NST ? 0 : cur + 1;
         if constexpr (WHOLE) {
             read(cur, 1, fa[1], fb[1]);
             product(fa[0], fb[0]);
@@ -221,16 +253,18 @@ __global__ __launch_bounds__(64 * WAVES_N * WAVES_M, 2) void tile_kernel(const A
                 __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
             }
             if constexpr (MORE) {
-                conv::wait_vmcnt<0>();
+                // the next stage has landed once only the stages behind it are in flight
+                if constexpr (REFILL) conv::wait_vmcnt<(NST - 2) * L>();
+                else conv::wait_vmcnt<0>();
                 conv::wait_lgkmcnt<0>();
                 __builtin_amdgcn_s_barrier();
                 asm volatile("" ::: "memory");
-                if constexpr (REFILL) issue(cur, kt + 2);
-                read(cur ^ 1, 0, fa[0], fb[0]);
+                if constexpr (REFILL) issue(cur, kt + NST);
+                read(next, 0, fa[0], fb[0]);
             }
             product(fa[1], fb[1]);
             if constexpr (MORE) {
-                if constexpr (REFILL) __builtin_amdgcn_sched_group_barrier(0x020, LW + LX, 0);
+                if constexpr (REFILL) __builtin_amdgcn_sched_group_barrier(0x020, L, 0);
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
 #pragma unroll
                 for (int r = 0; r < FN + FM; ++r) {
@@ -241,37 +275,37 @@ __global__ __launch_bounds__(64 * WAVES_N * WAVES_M, 2) void tile_kernel(const A
         } else {
             product(fa[0], fb[0]);
         }
+        cur = next;
     };
     constexpr std::true_type Y{};
     constexpr std::false_type N{};
     int kt = 0;
-    for (; kt + 2 < nk; ++kt) stage_step(Y, Y, Y, kt);
-    if (kt + 1 < nk) stage_step(N, Y, Y, kt++);
+    for (; kt + NST < nk; ++kt) stage_step(Y, Y, Y, kt);
+    for (; kt + 1 < nk; ++kt) stage_step(N, Y, Y, kt);
     if (halves & 1) stage_step(N, N, N, kt);
     else stage_step(N, N, Y, kt);
 
-    // lane (q, p): pixel p of every pixel fragment, channels 16 q .. + 15 of every 64-channel group
+    // lane (q, p): pixel p of every pixel fragment
+    using R = Run<OUT, 4>;
     const int q = lane >> 4, p = lane & 15, mw = m0 + wm * WM + p;
     float xs[FM];
 #pragma unroll
-    for (int j = 0; j < FM; ++j) xs[j] = mw + j * 16 < a.M ? a.xs[mw + j * 16] : 0.f;
+    for (int j = 0; j < FM; ++j) xs[j] = sc[2 * BN + wm * WM + j * 16 + p];
     with_mode(a, [&](auto mode) {
         using M = decltype(mode);
 #pragma unroll
         for (int g = 0; g < FN / 4; ++g) {
-            const int n = n0 + wn * WN + g * 64 + q * 16;
+            const int nl = wn * WN + g * 64 + q * R::PE, n = n0 + nl;
             float ws[16], bias[16];
-            load_channels<16>(a, n, ws, bias);
-            Run<OUT, 16> run[FM];
+            load_channels<R>(sc + nl, sc + BN + nl, ws, bias);
+            R run[FM];
 #pragma unroll
             for (int j = 0; j < FM; ++j) run[j].template load_residual<M>(a, mw + j * 16, n);
 #pragma unroll
             for (int j = 0; j < FM; ++j) {
                 int v[16];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[i * 4 + e] = acc[g * 4 + i][j][e];
+                for (int i = 0; i < 16; ++i) v[i] = acc[g * 4 + (i >> 2)][j][i & 3];
                 run[j].template store<M>(a, mw + j * 16, n, xs[j], v, ws, bias);
             }
         }
@@ -310,9 +344,9 @@ __global__ __launch_bounds__(64 * NW) void few_rows_kernel(const Args a) {
     const int n0 = (int)(t % (unsigned)a.tiles_n) * (16 * FN), m0 = (int)(t / (unsigned)a.tiles_n) * (16 * FM);
     const char* pw[FN];
     const char* px[FM];
-    // MFMA row (q, e) of fragment i is channel (q, i, e): a lane ends with 4 FN consecutive channels of its pixel
+    using R = Run<OUT, FN>;
 #pragma unroll
-    for (int i = 0; i < FN; ++i) pw[i] = a.w + (long long)(n0 + (p >> 2) * (4 * FN) + i * 4 + (p & 3)) * a.kp;
+    for (int i = 0; i < FN; ++i) pw[i] = a.w + (long long)(n0 + channel_of<R::PE>(i, p >> 2, p & 3)) * a.kp;
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
         const int m = m0 + j * 16 + p;
@@ -357,29 +391,29 @@ __global__ __launch_bounds__(64 * NW) void few_rows_kernel(const Args a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[i * 4 + e] = s[e];
         }
-        const int m = m0 + j * 16 + p, n = n0 + q * 4 * FN;
+        const int m = m0 + j * 16 + p, n = n0 + q * R::PE;
         float ws[4 * FN], bias[4 * FN];
-        load_channels<4 * FN>(a, n, ws, bias);
+        load_channels<R>(a.ws + n, a.bias ? a.bias + n : nullptr, ws, bias);
         with_mode(a, [&](auto mode) {
             using M = decltype(mode);
-            Run<OUT, 4 * FN> run;
+            R run;
             run.template load_residual<M>(a, m, n);
             run.template store<M>(a, m, n, m < a.M ? a.xs[m] : 0.f, v, ws, bias);
         });
     }
 }
 
-template <typename OUT, int BN, int BM, int WAVES_N, int WAVES_M>
+template <typename OUT, int BN, int BM, int WAVES_N, int WAVES_M, int NST = 2>
 static int launch_tile(Args a, hipStream_t stream) {
-    constexpr int most = 2 * (BN + BM) * 128;
-    const int lds = a.kp <= 128 ? most / 2 : most;      // (a single stage leaves room for twice the workgroups)
+    constexpr int scales = (2 * BN + BM) * 4, stage = (BN + BM) * 128, most = scales + NST * stage;
+    const int used = (a.kp + 127) / 128, lds = scales + (used < NST ? used : NST) * stage;      // (fewer stages leave room for more workgroups)
     a.tiles_n = (a.N + BN - 1) / BN;
     const long long blocks = (long long)a.tiles_n * ((a.M + BM - 1) / BM);
     YDET_CHECK_ARG(blocks * 64 * WAVES_N * WAVES_M <= UINT32_MAX, "matmul_i8: %d rows x %d channels are too many tiles", a.M, a.N);
     static unsigned char done[kMaxDevices];
-    const int rc = raise_dynamic_lds_limit(reinterpret_cast<const void*>(&tile_kernel<OUT, BN, BM, WAVES_N, WAVES_M>), most, done, "matmul_i8");
+    const int rc = raise_dynamic_lds_limit(reinterpret_cast<const void*>(&tile_kernel<OUT, BN, BM, WAVES_N, WAVES_M, NST>), most, done, "matmul_i8");
     if (rc != YDET_OK) return rc;
-    hipLaunchKernelGGL((tile_kernel<OUT, BN, BM, WAVES_N, WAVES_M>), dim3((unsigned)blocks), dim3(64 * WAVES_N * WAVES_M), lds, stream, a);
+    hipLaunchKernelGGL((tile_kernel<OUT, BN, BM, WAVES_N, WAVES_M, NST>), dim3((unsigned)blocks), dim3(64 * WAVES_N * WAVES_M), lds, stream, a);
     YDET_CHECK_LAUNCH("matmul_i8");
     return YDET_OK;
 }
@@ -394,13 +428,23 @@ static int launch_few(Args a, hipStream_t stream) {
     return YDET_OK;
 }
 
+// Which kernel takes a product, by rows, channels and K alone; every one gives the same bits.  Measured on 256 CUs, us:
+//   up to 16 rows, or rows that are not 16-byte aligned: straight from memory.
+//   256 x 192 tiles for K >= 2048 where they leave no quarter of the CUs idle (23104 x 4096 -> 512: 52, in 128 x 128 tiles 73; but
+//     25600 x 1024 -> 512: 32 against 25);
+//   128 x 128 for K >= 1024 with at least a tile a CU (6400 x 1024 -> 1024: 14.1, in 64 x 128 tiles 16.4);
+//   64 x 128 otherwise (409600 x 64 -> 64: 18, in 128 x 128 tiles 28; 409600 x 128 -> 128 with residual: 52 against 62), with a
+//     third stage where there are fewer than two workgroups a CU (2888 x 4096 -> 512: 14.6, with two stages 19.2).
 template <typename OUT>
 static int launch(const Args& a, bool wide_x, hipStream_t stream) {
     if (!wide_x) return a.M <= 16 ? launch_few<OUT, 1, 1, 8, true>(a, stream) : launch_few<OUT, 2, 2, 8, true>(a, stream);
-    const long long t128 = (long long)((a.M + 127) / 128) * ((a.N + 127) / 128);
     if (a.M <= 16) return launch_few<OUT, 1, 1, 8, false>(a, stream);
-    if (t128 < current_device_info().cus / 2) return launch_few<OUT, 2, 2, 8, false>(a, stream);
-    return launch_tile<OUT, 128, 128, 2, 2>(a, stream);
+    const int cus = current_device_info().cus;
+    auto tiles = [&](int bn, int bm) { return (long long)((a.N + bn - 1) / bn) * ((a.M + bm - 1) / bm); };
+    if (a.K >= 2048 && a.N > 128 && tiles(256, 192) * 4 >= cus * 3) return launch_tile<OUT, 256, 192, 2, 4>(a, stream);
+    if (a.K >= 1024 && a.N > 64 && tiles(128, 128) >= cus) return launch_tile<OUT, 128, 128, 2, 2>(a, stream);
+    if (tiles(64, 128) < 2 * cus) return launch_tile<OUT, 64, 128, 1, 4, 3>(a, stream);
+    return launch_tile<OUT, 64, 128, 1, 4, 2>(a, stream);
 }
 
 }  // namespace i8
@@ -440,6 +484,30 @@ int ydet_launch_matmul_i8(const ydet_matmul_i8_desc* d, hipStream_t stream) {
     // rows read in 16-byte pieces: the last piece of a row may reach behind K, so the pitch has to hold it
     const bool wide_x = (uintptr_t)a.x % 16 == 0 && d->x_ld % 16 == 0 && d->x_coff + (d->K + 15) / 16 * 16 <= d->x_ld;
     return d->out_dtype == YDET_BF16 ? i8::launch<__bf16>(a, wide_x, stream) : i8::launch<float>(a, wide_x, stream);
+}
+
+extern "C" size_t ydet_linear_i8_workspace_bytes(int64_t rows, int K) {
+    if (rows < 0 || K <= 0) return 0;
+    return (size_t)rows * ((K + 15) / 16 * 16) + (size_t)(rows + 3) / 4 * 16;
+}
+
+extern "C" int ydet_linear_i8(const ydet_quantize_desc* in, const ydet_matmul_i8_desc* product, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+    clear_error();
+    YDET_CHECK_ARG(in && product, "linear_i8: null descriptor");
+    YDET_CHECK_ARG(in->rows == product->rows && in->C == product->K, "linear_i8: %lld x %d rows for a product of %lld x %d", (long long)in->rows,
+                   in->C, (long long)product->rows, product->K);
+    if (in->rows == 0) return YDET_OK;
+    const size_t need = ydet_linear_i8_workspace_bytes(in->rows, in->C);
+    YDET_CHECK_ARG(need > 0 && workspace && (uintptr_t)workspace % 16 == 0, "linear_i8: needs a 16-byte aligned workspace");
+    if (workspace_bytes < need) return fail(YDET_ERR_WORKSPACE, "linear_i8: workspace %zu < %zu bytes", workspace_bytes, need);
+    ydet_quantize_desc q = *in;
+    ydet_matmul_i8_desc p = *product;
+    q.q_ld = p.x_ld = (in->C + 15) / 16 * 16, p.x_coff = 0;
+    p.x = q.q = static_cast<int8_t*>(workspace);
+    p.x_scale = q.scale = reinterpret_cast<float*>(q.q + in->rows * q.q_ld);
+    const int rc = ydet_launch_quantize_rows(&q, as_stream(stream));
+    return rc != YDET_OK ? rc : ydet_launch_matmul_i8(&p, as_stream(stream));
 }
 
 extern "C" int ydet_matmul_i8(const ydet_matmul_i8_desc* d, void* stream) {

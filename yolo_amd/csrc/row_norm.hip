@@ -6,7 +6,9 @@
 //
 // One pass over memory: a row is read once into the registers of the lanes that share it (rows_common.h), mean, variance
 // (from the differences to the mean, not as a difference of squares) and maximum are taken there, and the result is
-// written.  About ten operations a value against two to eight bytes: bound by HBM.  Sums, statistics and scales are in 32 bits.
+// written.  Sums, statistics and scales are in 32 bits.  The bytes of a bf16 value (2 in, 1 or 2 out) take as long as about
+// fifteen operations, so what is done once a row counts as well: rstd is the hardware's reciprocal square root, 1 / s its
+// reciprocal (one unit in the last place each), mean and scale are divided by a product and a remainder.
 #include "rows_common.h"
 
 namespace ydet {
@@ -24,10 +26,17 @@ struct RowArgs {
     int C, cw;          // values of a row; values written of a row (8-bit rows: zeros behind C)
     int x_ld, y_ld;
     int param_dtype;
-    float eps;
+    float eps, inv_c;
 };
 
 enum { kNorm = 1, kQuant = 2 };
+
+// a / b rounded once, with y the nearest number to 1 / b.  Markstein's step: q = a y, then q + (a - b q) y rounded once is the nearest
+// number to the quotient, as long as the remainder is exact, which tiny a do not allow.
+__device__ __forceinline__ float quotient(float a, float b, float y) {
+    const float q = a * y;
+    return fmaf(fmaf(-b, q, a), y, q);
+}
 
 // Nearest integer to v / s (ties to even), exactly, as a float's bits whose low byte is the integer.  The product with 1 / s
 // is within 3e-5 of the quotient, so rounding it (adding 1.5 * 2^23 leaves the integer in the low bits) is right unless it
@@ -86,7 +95,7 @@ __global__ __launch_bounds__(kThreads) void row_norm_kernel(const RowArgs a) {
                 float sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < CH * VEC; ++i) sum += v[i];
-                const float mean = group_sum<LPR>(sum, red, slot) / fc;
+                const float mean = quotient(group_sum<LPR>(sum, red, slot), fc, a.inv_c);
                 float sq = 0.f;
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
@@ -98,7 +107,7 @@ __global__ __launch_bounds__(kThreads) void row_norm_kernel(const RowArgs a) {
                         sq = fmaf(d, d, sq);
                     }
                 }
-                const float rstd = 1.f / sqrtf(group_sum<LPR>(sq, red, slot) / fc + a.eps);
+                const float rstd = __builtin_amdgcn_rsqf(fmaf(group_sum<LPR>(sq, red, slot), a.inv_c, a.eps));
                 if (a.mean && live && l == 0) {
                     a.mean[row] = mean;
                     a.rstd[row] = rstd;
@@ -133,7 +142,7 @@ __global__ __launch_bounds__(kThreads) void row_norm_kernel(const RowArgs a) {
                 const float amax = __uint_as_float(top);
                 const bool bad = top >= 0x7f800000u;                 // the row has no scale: NaN, and zeros
                 const bool some = !bad && amax >= 127.f * 1.17549435e-38f;   // smaller rows count as zero: s stays a normal number
-                const float s = some ? amax / 127.f : 1.f, inv = 1.f / s;
+                const float s = !some ? 1.f : amax < 1e-25f ? amax / 127.f : quotient(amax, 127.f, 1.f / 127.f), inv = __builtin_amdgcn_rcpf(s);
                 if (live && l == 0) a.scale[row] = some ? s : bad ? __uint_as_float(0x7fc00000u) : 0.f;
                 unsigned m[CH * VEC];
                 float near = 0.f;
@@ -238,7 +247,7 @@ int ydet_launch_layer_norm(const ydet_layer_norm_desc* d, hipStream_t stream) {
     YDET_CHECK_ARG(((uintptr_t)a.x | (uintptr_t)a.y) % es == 0, "layer_norm: misaligned tensor");
     a.gamma = static_cast<const char*>(d->gamma), a.beta = static_cast<const char*>(d->beta);
     a.mean = d->mean, a.rstd = d->rstd, a.rows = d->rows, a.C = a.cw = d->C;
-    a.x_ld = d->x_ld, a.y_ld = d->y_ld, a.param_dtype = d->param_dtype, a.eps = d->eps;
+    a.x_ld = d->x_ld, a.y_ld = d->y_ld, a.param_dtype = d->param_dtype, a.eps = d->eps, a.inv_c = 1.f / (float)d->C;
     return launch_mode<kNorm>(a, d->dtype, stream);
 }
 
@@ -262,7 +271,7 @@ int ydet_launch_quantize_rows(const ydet_quantize_desc* d, hipStream_t stream) {
     YDET_CHECK_ARG((uintptr_t)a.x % es == 0 && (uintptr_t)a.y % 16 == 0, "quantize_rows: misaligned tensor");
     a.scale = d->scale, a.rows = d->rows, a.C = d->C, a.cw = cw, a.x_ld = d->x_ld, a.y_ld = d->q_ld;
     a.gamma = static_cast<const char*>(d->gamma), a.beta = static_cast<const char*>(d->beta);
-    a.param_dtype = d->param_dtype, a.eps = d->eps;
+    a.param_dtype = d->param_dtype, a.eps = d->eps, a.inv_c = 1.f / (float)d->C;
     return d->normalize ? launch_mode<kNorm | kQuant>(a, d->dtype, stream) : launch_mode<kQuant>(a, d->dtype, stream);
 }
 

@@ -505,54 +505,80 @@ _ACTS = {"none": _ffi.ACT_NONE, "leaky": _ffi.ACT_LEAKY, "silu": _ffi.ACT_SILU}
 _RES = {"after": _ffi.RES_AFTER_ACT, "before": _ffi.RES_BEFORE_ACT}
 
 
-def matmul_i8(q, scale, lin, act="none", slope=0.1, res=None, res_mode="after", out_dtype=torch.bfloat16):
-    """act(q . lin.w^T * scale * lin.scale + lin.bias), [..., N] of out_dtype (bf16 or fp32), from int8 rows q [..., K] and
-    their scales [...] (quantize_rows).  act: "none", "leaky" (negative slope `slope`), "silu".  res [..., N] of out_dtype is
-    added after or before the activation (res_mode).  The sums are exact integers."""
-    _need_cuda(q, scale)
-    lib = _ffi.lib()
+def _product(x, scale, n, ld, lin, act, slope, res, res_mode, out_dtype):
+    """(output, descriptor, what it points to) of a product with `lin`; x, scale: addresses of n 8-bit rows and their scales."""
     if act not in _ACTS or res_mode not in _RES:
         raise ValueError(f"act {act!r} / res_mode {res_mode!r}: want one of {sorted(_ACTS)} / {sorted(_RES)}")
-    if q.dtype != torch.int8 or q.dim() == 0 or q.shape[-1] != lin.K:
-        raise ValueError(f"q is int8 [..., {lin.K}]: got {q.dtype} {tuple(q.shape)}")
-    dev, lead = q.device, q.shape[:-1]
-    if scale.shape != lead or scale.dtype != torch.float32:
-        raise ValueError(f"scale is fp32 {tuple(lead)}: got {scale.dtype} {tuple(scale.shape)}")
     if out_dtype == torch.bfloat16:
         odt = _ffi.BF16
     elif out_dtype == torch.float32:
         odt = _ffi.F32
     else:
         raise TypeError(f"unsupported dtype {out_dtype}")
-    if dev != lin.device or dev != scale.device or (res is not None and dev != res.device):
-        raise RuntimeError("matmul_i8: tensors on different devices")
-    q, n, ld = _as_rows(q, "matmul_i8")
-    if ld > 1 << 23:
-        q, ld = q.contiguous(), lin.K
-    # the library may read a row's last piece up to its 16-byte border: a view whose storage ends before that is copied
-    K16 = (lin.K + 15) // 16 * 16
-    if n and K16 != lin.K and ld % 16 == 0 and q.data_ptr() % 16 == 0 \
-            and q.storage_offset() + (n - 1) * ld + K16 > q.untyped_storage().nbytes():
-        q, ld = q.contiguous(), lin.K
-    scale = scale.contiguous()
+    N, dev = lin.N, lin.device
     rmode, rptr, r_ld = _ffi.RES_NONE, None, 0
     if res is not None:
-        if res.shape != lead + (lin.N,) or res.dtype != out_dtype:
-            raise ValueError(f"res is {out_dtype} {tuple(lead) + (lin.N,)}: got {res.dtype} {tuple(res.shape)}")
-        res, _, r_ld = _as_rows(res.detach(), "matmul_i8")
+        if res.shape[-1:] != (N,) or res.numel() != n * N or res.dtype != out_dtype:
+            raise ValueError(f"res is {out_dtype} of {n} rows of {N} channels: got {res.dtype} {tuple(res.shape)}")
+        if res.device != dev:
+            raise RuntimeError(f"res on {res.device}, the weights on {dev}")
+        res, _, r_ld = _as_rows(res, "matmul_i8")
         rmode, rptr = _RES[res_mode], res.data_ptr()
-    y = torch.empty(lead + (lin.N,), device=dev, dtype=out_dtype)
-    d = _ffi.MatmulI8Desc(q.data_ptr(), scale.data_ptr(), lin.w.data_ptr(), lin.scale.data_ptr(), _ptr(lin.bias), rptr, y.data_ptr(),
-                          n, lin.K, lin.N, lin.kp, lin.n_pad, ld, 0, lin.N, 0, r_ld, 0, _ACTS[act], slope, rmode, odt)
-    rc = _launch(dev, lib.ydet_matmul_i8, d)
+    y = torch.empty((n, N), device=dev, dtype=out_dtype)
+    return y, _ffi.MatmulI8Desc(x, scale, lin.w.data_ptr(), lin.scale.data_ptr(), _ptr(lin.bias), rptr, y.data_ptr(), n, lin.K, N, lin.kp,
+                                lin.n_pad, ld, 0, N, 0, r_ld, 0, _ACTS[act], slope, rmode, odt), res
+
+
+def matmul_i8(q, scale, lin, act="none", slope=0.1, res=None, res_mode="after", out_dtype=torch.bfloat16):
+    """act(q . lin.w^T * scale * lin.scale + lin.bias), [..., N] of out_dtype (bf16 or fp32), from int8 rows q [..., K] and
+    their scales [...] (quantize_rows).  act: "none", "leaky" (negative slope `slope`), "silu".  res [..., N] of out_dtype is
+    added after or before the activation (res_mode).  The sums are exact integers."""
+    _need_cuda(q, scale)
+    K, shape = lin.K, q.shape
+    if q.dtype != torch.int8 or len(shape) == 0 or shape[-1] != K:
+        raise ValueError(f"q is int8 [..., {K}]: got {q.dtype} {tuple(shape)}")
+    lead = shape[:-1]
+    if scale.shape != lead or scale.dtype != torch.float32:
+        raise ValueError(f"scale is fp32 {tuple(lead)}: got {scale.dtype} {tuple(scale.shape)}")
+    if res is not None and res.shape[:-1] != lead:
+        raise ValueError(f"res is [..., {lin.N}] with q's leading dimensions {tuple(lead)}: got {tuple(res.shape)}")
+    dev = q.device
+    if dev != lin.device or dev != scale.device:
+        raise RuntimeError("matmul_i8: tensors on different devices")
+    q, n, ld = _as_rows(q, "matmul_i8")
+    # the library may read a row's last piece up to its 16-byte border: a view whose storage ends before that is copied
+    if ld > 1 << 23 or (K % 16 and ld % 16 == 0 and n and q.data_ptr() % 16 == 0 and
+                        q.storage_offset() + (n - 1) * ld + (K + 15) // 16 * 16 > q.untyped_storage().nbytes()):
+        q, ld = q.clone(memory_format=torch.contiguous_format), K
+    if not scale.is_contiguous():
+        scale = scale.contiguous()
+    y, d, keep = _product(q.data_ptr(), scale.data_ptr(), n, ld, lin, act, slope, res, res_mode, out_dtype)
+    rc = _launch(dev, _ffi.lib().ydet_matmul_i8, d)
     if rc:
         _ffi.check(rc, "ydet_matmul_i8")
-    return y
+    return y if len(lead) == 1 else y.view(lead + (lin.N,))
 
 
 def linear_i8(x, lin, act="none", slope=0.1, res=None, res_mode="after", out_dtype=None):
-    """matmul_i8 of a floating map x [..., K], whose rows are quantised on the way; out_dtype defaults to x's."""
-    if x.shape[-1:] != (lin.K,):
-        raise ValueError(f"x is [..., {lin.K}]: got {tuple(x.shape)}")
-    q, scale = quantize_rows(x)
-    return matmul_i8(q, scale, lin, act, slope, res, res_mode, x.dtype if out_dtype is None else out_dtype)
+    """matmul_i8 of a floating map x [..., K], whose rows are quantised (quantize_rows) on the way; out_dtype defaults to x's."""
+    _need_cuda(x)
+    K, shape = lin.K, x.shape
+    if shape[-1:] != (K,):
+        raise ValueError(f"x is [..., {K}]: got {tuple(shape)}")
+    lead = shape[:-1]
+    if res is not None and res.shape[:-1] != lead:
+        raise ValueError(f"res is [..., {lin.N}] with x's leading dimensions {tuple(lead)}: got {tuple(res.shape)}")
+    dev = x.device
+    if dev != lin.device:
+        raise RuntimeError("linear_i8: tensors on different devices")
+    lib = _ffi.lib()
+    dt = _dt(x)
+    x, n, ld = _as_rows(x, "linear_i8")
+    y, d, keep = _product(None, None, n, 0, lin, act, slope, res, res_mode, x.dtype if out_dtype is None else out_dtype)
+    nbytes = lib.ydet_linear_i8_workspace_bytes(n, K)
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    src = _ffi.QuantizeDesc(x.data_ptr(), None, None, None, None, n, K, ld, 0, 0, dt, _ffi.F32, 0, 0.0)
+    rc = _launch(dev, lib.ydet_linear_i8, src, d, ws.data_ptr(), nbytes)
+    if rc:
+        _ffi.check(rc, "ydet_linear_i8")
+    return y if len(lead) == 1 else y.view(lead + (lin.N,))
