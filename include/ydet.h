@@ -525,9 +525,10 @@ int ydet_quantize_rows_i8(const ydet_quantize_desc* d, void* stream);
  *   acc[r, n] = sum_k x[r, k] * w[n, k]      (exact 32-bit integers; K <= 131071)
  *   y[r, n]   = act(acc * x_scale[r] * w_scale[n] + bias[n])  with the residual as in ydet_conv2d_nhwc (res_mode; res has y's dtype)
  * w [n_pad][kp], rows >= N and columns >= K zero, n_pad a multiple of 128, kp a multiple of 64; w_scale and bias (may be NULL)
- * hold n_pad values; all three 16-byte aligned.  x may lie anywhere; slices that are 16-byte aligned with x_ld a multiple
- * of 16 are read in 16-byte pieces (the bytes behind K in a row's last piece are read, their values do not matter; the
- * slice's row has to hold them).  y may be res.  x_ld <= 2^23, rows < 2^31 - 512. */
+ * hold n_pad values; all three 16-byte aligned.  Slices that are 16-byte aligned with x_ld a multiple of 16 are read in
+ * 16-byte pieces (the bytes behind K in a row's last piece are read, their values do not matter; the slice's row has to hold
+ * them); x may lie anywhere else too, and then many rows need ydet_matmul_i8_workspace_bytes(d) bytes of workspace (16-byte
+ * aligned; 0: none, also for a descriptor that ydet_matmul_i8 refuses).  y may be res.  x_ld <= 2^23, rows < 2^31 - 512. */
 typedef struct {
     const int8_t* x;
     const float* x_scale;
@@ -544,7 +545,8 @@ typedef struct {
     int32_t res_mode; /* ydet_res_mode */
     int32_t out_dtype;/* dtype of y and res */
 } ydet_matmul_i8_desc;
-int ydet_matmul_i8(const ydet_matmul_i8_desc* d, void* stream);
+size_t ydet_matmul_i8_workspace_bytes(const ydet_matmul_i8_desc* d);
+int ydet_matmul_i8(const ydet_matmul_i8_desc* d, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ydet_quantize_rows_i8 and ydet_matmul_i8 behind each other, the 8-bit rows in the caller's workspace
  * (ydet_linear_i8_workspace_bytes(rows, K), 16-byte aligned): `in` without q, scale and q_ld, `product` without x, x_scale, x_ld

@@ -399,7 +399,7 @@ def test_rows_beyond_32_bit_offsets():
     # the library's own slices: output rows that far apart
     d = _ffi.MatmulI8Desc(q.data_ptr(), s.data_ptr(), lin.w.data_ptr(), lin.scale.data_ptr(), None, None, big.data_ptr(), rows, 64, 48,
                           lin.kp, lin.n_pad, 64, 0, ld, 1024, 0, 0, 0, 0.0, 0, _ffi.BF16)
-    _ffi.check(_ffi.lib().ydet_matmul_i8(d, _ffi.current_stream()))
+    _ffi.check(_ffi.lib().ydet_matmul_i8(d, None, 0, _ffi.current_stream()))
     assert torch.equal(big[:, 1024:1072], want)
 
 

@@ -50,7 +50,7 @@ def product(**kw):
     d = dict(x=P, x_scale=P, w=P, w_scale=P, bias=P, res=None, y=P, rows=4, K=64, N=32, kp=64, n_pad=128, x_ld=64, x_coff=0, y_ld=32,
              y_coff=0, res_ld=0, res_coff=0, act=0, slope=0.0, res_mode=0, out_dtype=1)
     d.update(kw)
-    return _ffi.lib().ydet_matmul_i8(_ffi.MatmulI8Desc(**d), None)
+    return _ffi.lib().ydet_matmul_i8(_ffi.MatmulI8Desc(**d), None, 0, None)
 
 
 ARG, WS = -1, -3

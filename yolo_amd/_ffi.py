@@ -175,7 +175,8 @@ SYMBOLS = {
     "ydet_quantize_rows_i8": (C.c_int, [C.POINTER(QuantizeDesc), C.c_void_p]),
     "ydet_linear_i8_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int]),
     "ydet_linear_i8": (C.c_int, [C.POINTER(QuantizeDesc), C.POINTER(MatmulI8Desc), C.c_void_p, C.c_size_t, C.c_void_p]),
-    "ydet_matmul_i8": (C.c_int, [C.POINTER(MatmulI8Desc), C.c_void_p]),
+    "ydet_matmul_i8_workspace_bytes": (C.c_size_t, [C.POINTER(MatmulI8Desc)]),
+    "ydet_matmul_i8": (C.c_int, [C.POINTER(MatmulI8Desc), C.c_void_p, C.c_size_t, C.c_void_p]),
     "ydet_run_ops": (C.c_int, [C.POINTER(Op), C.c_int, C.c_void_p]),
     "ydet_run_op_lists": (C.c_int, [C.POINTER(C.POINTER(Op)), C.POINTER(C.c_int), C.c_int, C.c_void_p]),
     "ydet_timer_create": (C.c_void_p, [C.c_int]),

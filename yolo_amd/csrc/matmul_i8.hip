@@ -26,7 +26,6 @@ struct Args {
     long long x_ld, y_ld, res_ld;
     int act, res_mode;
     float slope;
-    int vec;                // 16-byte stores and residual loads are legal (and N is a multiple of the run of channels a lane holds)
     int tiles_n;
 };
 
@@ -76,6 +75,7 @@ template <typename OUT, int F>
 struct Run {
     static constexpr int PE = F == 1 ? 4 : 16 / (int)sizeof(OUT), NP = 4 * F / PE, C = 4 * F;
     typedef OUT piece __attribute__((ext_vector_type(PE)));
+    typedef piece loose __attribute__((aligned(sizeof(OUT))));      // (gfx950 moves 16 bytes from and to any address)
     piece r[NP];        // the residual
 
     template <typename M>
@@ -85,14 +85,13 @@ struct Run {
 #pragma unroll
             for (int k = 0; k < NP; ++k) {
                 r[k] = piece{};
-                if (m < a.M && n + 4 * PE * k < a.N) {
-                    if (a.vec) {
-                        r[k] = *reinterpret_cast<const piece*>(p + 4 * PE * k);
-                    } else {
+                if (m >= a.M) continue;
+                if (n + 4 * PE * k + PE <= a.N) {
+                    r[k] = *reinterpret_cast<const loose*>(p + 4 * PE * k);
+                } else {
 #pragma unroll
-                        for (int e = 0; e < PE; ++e)
-                            if (n + 4 * PE * k + e < a.N) r[k][e] = p[4 * PE * k + e];
-                    }
+                    for (int e = 0; e < PE - 1; ++e)
+                        if (n + 4 * PE * k + e < a.N) r[k][e] = p[4 * PE * k + e];
                 }
             }
         }
@@ -111,11 +110,11 @@ struct Run {
                 if constexpr (M::res != YDET_RES_NONE) rr = (float)r[k][e];
                 o[e] = (OUT)finish<M>(fmaf((float)acc[k * PE + e] * xs, ws[k * PE + e], bias[k * PE + e]), rr, a);
             }
-            if (a.vec) {
-                if (n + 4 * PE * k < a.N) *reinterpret_cast<piece*>(y + 4 * PE * k) = o;
+            if (n + 4 * PE * k + PE <= a.N) {
+                *reinterpret_cast<loose*>(y + 4 * PE * k) = o;
             } else {
 #pragma unroll
-                for (int e = 0; e < PE; ++e)
+                for (int e = 0; e < PE - 1; ++e)
                     if (n + 4 * PE * k + e < a.N) y[4 * PE * k + e] = o[e];
             }
         }
@@ -315,24 +314,22 @@ __global__ __launch_bounds__(64 * WAVES_N * WAVES_M, 2) void tile_kernel(const A
 // ---- few rows: the K of a small tile is shared by the waves of a workgroup ------------------------------------------------
 // 16 FN channels x 16 FM pixels a workgroup; each of its NW waves takes every NW-th 64 bytes of K, its operands straight
 // from memory into registers (all loads of a wave in flight together: the call costs one or two memory latencies), and the
-// waves' integer sums meet in LDS.  ANY: rows of x at any byte address and pitch (K need not be padded).
+// waves' integer sums meet in LDS.  ANY: rows of x at any byte address and pitch.  Pieces may reach behind a row's K (the weights
+// are zero there), but not behind the last row's: `left` bytes of x lie from p on.
 template <bool ANY>
-__device__ __forceinline__ i32x4 load_k16(const char* p, int k, int K) {
-    if constexpr (!ANY) {
-        return k < K ? *reinterpret_cast<const i32x4*>(p + k) : i32x4{0, 0, 0, 0};
+__device__ __forceinline__ i32x4 load_k16(const char* p, long long left) {
+    if constexpr (!ANY) return *reinterpret_cast<const i32x4*>(p);
+    i32x4 v{0, 0, 0, 0};
+    if (left >= 16) {
+        __builtin_memcpy(&v, p, 16);
     } else {
-        i32x4 v{0, 0, 0, 0};
-        if (k + 16 <= K) {
-            __builtin_memcpy(&v, p + k, 16);
-        } else if (k < K) {
-            unsigned u[4] = {0u, 0u, 0u, 0u};
+        unsigned u[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-            for (int i = 0; i < 15; ++i)
-                if (k + i < K) u[i >> 2] |= (unsigned)(unsigned char)p[k + i] << (8 * (i & 3));
-            v = i32x4{(int)u[0], (int)u[1], (int)u[2], (int)u[3]};
-        }
-        return v;
+        for (int i = 0; i < 15; ++i)
+            if (i < left) u[i >> 2] |= (unsigned)(unsigned char)p[i] << (8 * (i & 3));
+        v = i32x4{(int)u[0], (int)u[1], (int)u[2], (int)u[3]};
     }
+    return v;
 }
 
 template <typename OUT, int FN, int FM, int NW, bool ANY>
@@ -342,15 +339,17 @@ __global__ __launch_bounds__(64 * NW) void few_rows_kernel(const Args a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, p = lane & 15;
     const unsigned t = xcd_remap(blockIdx.x, gridDim.x);
     const int n0 = (int)(t % (unsigned)a.tiles_n) * (16 * FN), m0 = (int)(t / (unsigned)a.tiles_n) * (16 * FM);
+    using R = Run<OUT, FN>;
     const char* pw[FN];
     const char* px[FM];
-    using R = Run<OUT, FN>;
+    long long left[FM];
 #pragma unroll
     for (int i = 0; i < FN; ++i) pw[i] = a.w + (long long)(n0 + channel_of<R::PE>(i, p >> 2, p & 3)) * a.kp;
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
-        const int m = m0 + j * 16 + p;
-        px[j] = a.x + (long long)(m < a.M ? m : a.M - 1) * a.x_ld;
+        const int m = m0 + j * 16 + p < a.M ? m0 + j * 16 + p : a.M - 1;
+        px[j] = a.x + m * a.x_ld;
+        left[j] = (a.M - 1 - m) * a.x_ld + a.K;
     }
     i32x4 acc[FN][FM];
 #pragma unroll
@@ -367,7 +366,7 @@ __global__ __launch_bounds__(64 * NW) void few_rows_kernel(const Args a) {
 #pragma unroll
             for (int i = 0; i < FN; ++i) fa[u][i] = in ? *reinterpret_cast<const i32x4*>(pw[i] + k) : i32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int j = 0; j < FM; ++j) fb[u][j] = load_k16<ANY>(px[j], k, a.K);
+            for (int j = 0; j < FM; ++j) fb[u][j] = k < a.K ? load_k16<ANY>(px[j] + k, left[j] - k) : i32x4{0, 0, 0, 0};
         }
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u)
@@ -428,22 +427,42 @@ static int launch_few(Args a, hipStream_t stream) {
     return YDET_OK;
 }
 
+// Rows at any address and pitch into rows of K rounded up to 16, for the tile kernels (bytes behind K: anything).
+__global__ __launch_bounds__(256) void align_rows_kernel(const char* x, long long ld, int M, int K, char* to) {
+    const int pieces = (K + 15) / 16;
+    const long long all = (long long)M * pieces;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long long)gridDim.x * 256) {
+        const long long m = i / pieces;
+        const int k = (int)(i - m * pieces) * 16;
+        *reinterpret_cast<i32x4*>(to + i * 16) = load_k16<true>(x + m * ld + k, (M - 1 - m) * ld + K - k);
+    }
+}
+
 // Which kernel takes a product, by rows, channels and K alone; every one gives the same bits.  Measured on 256 CUs, us:
-//   up to 16 rows, or rows that are not 16-byte aligned: straight from memory.
+//   16 x 16 outputs a workgroup, straight from memory, up to two workgroups a CU (1 x 1024 -> 1024: 2.9; 40 x 4096 -> 512: 5.7, in
+//     64 x 128 tiles 12.2; 100 x 1024 -> 512: 3.3 against 5.3);
+//   32 x 32, straight from memory, up to one a CU (400 x 1024 -> 512: 4.6 against 5.4; 200 x 2048 -> 1024: 6.4 against 7.7, but
+//     1600 x 512 -> 512: 6.7 against 4.5);
 //   256 x 192 tiles for K >= 2048 where they leave no quarter of the CUs idle (23104 x 4096 -> 512: 52, in 128 x 128 tiles 73; but
 //     25600 x 1024 -> 512: 32 against 25);
 //   128 x 128 for K >= 1024 with at least a tile a CU (6400 x 1024 -> 1024: 14.1, in 64 x 128 tiles 16.4);
 //   64 x 128 otherwise (409600 x 64 -> 64: 18, in 128 x 128 tiles 28; 409600 x 128 -> 128 with residual: 52 against 62), with a
 //     third stage where there are fewer than two workgroups a CU (2888 x 4096 -> 512: 14.6, with two stages 19.2).
+// The tile kernels want rows in 16-byte pieces: others are first copied into the workspace.
+static long long tiles(const Args& a, int bn, int bm) { return (long long)((a.N + bn - 1) / bn) * ((a.M + bm - 1) / bm); }
+static int direct_size(const Args& a) {
+    const int cus = current_device_info().cus;
+    return tiles(a, 16, 16) <= 2 * cus ? 16 : tiles(a, 32, 32) <= cus ? 32 : 0;
+}
+
 template <typename OUT>
 static int launch(const Args& a, bool wide_x, hipStream_t stream) {
-    if (!wide_x) return a.M <= 16 ? launch_few<OUT, 1, 1, 8, true>(a, stream) : launch_few<OUT, 2, 2, 8, true>(a, stream);
-    if (a.M <= 16) return launch_few<OUT, 1, 1, 8, false>(a, stream);
-    const int cus = current_device_info().cus;
-    auto tiles = [&](int bn, int bm) { return (long long)((a.N + bn - 1) / bn) * ((a.M + bm - 1) / bm); };
-    if (a.K >= 2048 && a.N > 128 && tiles(256, 192) * 4 >= cus * 3) return launch_tile<OUT, 256, 192, 2, 4>(a, stream);
-    if (a.K >= 1024 && a.N > 64 && tiles(128, 128) >= cus) return launch_tile<OUT, 128, 128, 2, 2>(a, stream);
-    if (tiles(64, 128) < 2 * cus) return launch_tile<OUT, 64, 128, 1, 4, 3>(a, stream);
+    const int cus = current_device_info().cus, direct = direct_size(a);
+    if (direct == 16) return wide_x ? launch_few<OUT, 1, 1, 8, false>(a, stream) : launch_few<OUT, 1, 1, 8, true>(a, stream);
+    if (direct == 32) return wide_x ? launch_few<OUT, 2, 2, 4, false>(a, stream) : launch_few<OUT, 2, 2, 4, true>(a, stream);
+    if (a.K >= 2048 && a.N > 128 && tiles(a, 256, 192) * 4 >= cus * 3) return launch_tile<OUT, 256, 192, 2, 4>(a, stream);
+    if (a.K >= 1024 && a.N > 64 && tiles(a, 128, 128) >= cus) return launch_tile<OUT, 128, 128, 2, 2>(a, stream);
+    if (tiles(a, 64, 128) < 2 * cus) return launch_tile<OUT, 64, 128, 1, 4, 3>(a, stream);
     return launch_tile<OUT, 64, 128, 1, 4, 2>(a, stream);
 }
 
@@ -452,7 +471,8 @@ static int launch(const Args& a, bool wide_x, hipStream_t stream) {
 
 using namespace ydet;
 
-int ydet_launch_matmul_i8(const ydet_matmul_i8_desc* d, hipStream_t stream) {
+// Checks a descriptor and fills the launch arguments; wide_x: its rows can be read in 16-byte pieces.
+static int fill_args(const ydet_matmul_i8_desc* d, i8::Args& a, bool& wide_x) {
     YDET_CHECK_ARG(d, "matmul_i8: null descriptor");
     YDET_CHECK_ARG(d->rows >= 0 && d->rows <= INT32_MAX - 512 && d->K > 0 && d->K <= 131071 && d->N > 0 && d->N <= (1 << 24),
                    "matmul_i8: rows=%lld K=%d N=%d (K up to 131071: the sums are 32-bit integers)", (long long)d->rows, d->K, d->N);
@@ -466,11 +486,10 @@ int ydet_launch_matmul_i8(const ydet_matmul_i8_desc* d, hipStream_t stream) {
                    "matmul_i8: act %d res_mode %d", d->act, d->res_mode);
     YDET_CHECK_ARG(d->res_mode == YDET_RES_NONE || (d->res_coff >= 0 && (long long)d->res_coff + d->N <= d->res_ld),
                    "matmul_i8: the residual's slice lies outside its rows");
-    if (d->rows == 0) return YDET_OK;
-    YDET_CHECK_ARG(d->x && d->x_scale && d->w && d->w_scale && d->y && (d->res_mode == YDET_RES_NONE || d->res), "matmul_i8: null pointer");
+    YDET_CHECK_ARG(d->rows == 0 || (d->x && d->x_scale && d->w && d->w_scale && d->y && (d->res_mode == YDET_RES_NONE || d->res)), "matmul_i8: null pointer");
     YDET_CHECK_ARG(((uintptr_t)d->w | (uintptr_t)d->w_scale | (uintptr_t)d->bias) % 16 == 0, "matmul_i8: weights, scales and bias need 16-byte alignment");
     const size_t es = dtype_size(d->out_dtype);
-    i8::Args a{};
+    a = i8::Args{};
     a.x = reinterpret_cast<const char*>(d->x) + d->x_coff;
     a.xs = d->x_scale, a.w = reinterpret_cast<const char*>(d->w), a.ws = d->w_scale, a.bias = d->bias;
     a.y = static_cast<char*>(d->y) + d->y_coff * es;
@@ -479,11 +498,37 @@ int ydet_launch_matmul_i8(const ydet_matmul_i8_desc* d, hipStream_t stream) {
     YDET_CHECK_ARG(((uintptr_t)a.y | (uintptr_t)a.res) % es == 0 && (uintptr_t)a.xs % 4 == 0, "matmul_i8: misaligned tensor");
     a.M = (int)d->rows, a.K = d->K, a.N = d->N, a.kp = d->kp, a.n_pad = d->n_pad;
     a.x_ld = d->x_ld, a.y_ld = d->y_ld, a.res_ld = d->res_ld, a.act = d->act, a.slope = d->act == YDET_ACT_LEAKY ? d->slope : 1.f;
-    auto wide = [&](const char* p, int ld) { return (uintptr_t)p % 16 == 0 && ld * es % 16 == 0; };
-    a.vec = d->N % 16 == 0 && wide(a.y, d->y_ld) && (a.res_mode == YDET_RES_NONE || wide(a.res, d->res_ld));
-    // rows read in 16-byte pieces: the last piece of a row may reach behind K, so the pitch has to hold it
-    const bool wide_x = (uintptr_t)a.x % 16 == 0 && d->x_ld % 16 == 0 && d->x_coff + (d->K + 15) / 16 * 16 <= d->x_ld;
+    // (the last piece of a row may reach behind K, so the pitch has to hold it)
+    wide_x = (uintptr_t)a.x % 16 == 0 && d->x_ld % 16 == 0 && d->x_coff + (d->K + 15) / 16 * 16 <= d->x_ld;
+    return YDET_OK;
+}
+
+static size_t aligned_bytes(const i8::Args& a) { return (size_t)a.M * ((a.K + 15) / 16 * 16); }
+
+int ydet_launch_matmul_i8(const ydet_matmul_i8_desc* d, void* ws, size_t ws_bytes, hipStream_t stream) {
+    i8::Args a;
+    bool wide_x;
+    const int rc = fill_args(d, a, wide_x);
+    if (rc != YDET_OK || a.M == 0) return rc;
+    if (!wide_x && !i8::direct_size(a)) {
+        if (ws_bytes < aligned_bytes(a))
+            return fail(YDET_ERR_WORKSPACE, "matmul_i8: workspace %zu < %zu bytes", ws_bytes, aligned_bytes(a));
+        YDET_CHECK_ARG(ws && (uintptr_t)ws % 16 == 0, "matmul_i8: rows of %d at this address and pitch need a 16-byte aligned workspace", a.K);
+        const long long blocks = ((long long)(aligned_bytes(a) / 16) + 255) / 256;
+        hipLaunchKernelGGL(i8::align_rows_kernel, dim3((unsigned)(blocks < (1 << 20) ? blocks : (1 << 20))), dim3(256), 0, stream, a.x, a.x_ld, a.M,
+                           a.K, static_cast<char*>(ws));
+        YDET_CHECK_LAUNCH("matmul_i8 (rows)");
+        a.x = static_cast<const char*>(ws), a.x_ld = (a.K + 15) / 16 * 16, wide_x = true;
+    }
     return d->out_dtype == YDET_BF16 ? i8::launch<__bf16>(a, wide_x, stream) : i8::launch<float>(a, wide_x, stream);
+}
+
+extern "C" size_t ydet_matmul_i8_workspace_bytes(const ydet_matmul_i8_desc* d) {
+    clear_error();
+    i8::Args a;
+    bool wide_x;
+    if (fill_args(d, a, wide_x) != YDET_OK || wide_x || a.M == 0 || i8::direct_size(a)) return 0;
+    return aligned_bytes(a);
 }
 
 extern "C" size_t ydet_linear_i8_workspace_bytes(int64_t rows, int K) {
@@ -507,10 +552,10 @@ extern "C" int ydet_linear_i8(const ydet_quantize_desc* in, const ydet_matmul_i8
     p.x = q.q = static_cast<int8_t*>(workspace);
     p.x_scale = q.scale = reinterpret_cast<float*>(q.q + in->rows * q.q_ld);
     const int rc = ydet_launch_quantize_rows(&q, as_stream(stream));
-    return rc != YDET_OK ? rc : ydet_launch_matmul_i8(&p, as_stream(stream));
+    return rc != YDET_OK ? rc : ydet_launch_matmul_i8(&p, nullptr, 0, as_stream(stream));
 }
 
-extern "C" int ydet_matmul_i8(const ydet_matmul_i8_desc* d, void* stream) {
+extern "C" int ydet_matmul_i8(const ydet_matmul_i8_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
     clear_error();
-    return ydet_launch_matmul_i8(d, as_stream(stream));
+    return ydet_launch_matmul_i8(d, workspace, workspace_bytes, as_stream(stream));
 }
