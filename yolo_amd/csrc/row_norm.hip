@@ -181,18 +181,20 @@ __global__ __launch_bounds__(kThreads) void row_norm_kernel(const RowArgs a) {
     }
 }
 
+// Workgroups: each walks over rows, weight and bias in its registers.  No more than stay resident where a workgroup reads weight and
+// bias (23104 x 2048 norm + quantisation in bf16: 54 us with four a CU, 72 with one for every four rows; rows of up to 1024
+// values have room for eight a CU), twice as many where it reads none (25600 x 512 quantisation: 10.9 us, with eight 11.6) or
+// takes four rows at a time (409600 x 128 norm: 39.2 us, with eight 41.7).
 template <int MODE, typename T, bool RAG, int LPR, int CH, int RPT>
 static int launch_rows(const RowArgs& a, hipStream_t stream) {
-    constexpr int per = kThreads / LPR * RPT;
-    const long long need = (a.rows + per - 1) / per;
-    const unsigned blocks = (unsigned)(need < (1 << 20) ? need : (1 << 20));
-    hipLaunchKernelGGL((row_norm_kernel<MODE, T, RAG, LPR, CH, RPT>), dim3(blocks), dim3(kThreads), 0, stream, a);
+    constexpr int per = kThreads / LPR * RPT, per_cu = !(MODE & kNorm) || RPT > 1 ? 16 : CH * 16 / (int)sizeof(T) > 16 ? 4 : 8;
+    const long long need = (a.rows + per - 1) / per, most = (long long)current_device_info().cus * per_cu;
+    hipLaunchKernelGGL((row_norm_kernel<MODE, T, RAG, LPR, CH, RPT>), dim3((unsigned)(need < most ? need : most)), dim3(kThreads), 0, stream, a);
     YDET_CHECK_LAUNCH("row norm / quantise");
     return YDET_OK;
 }
 
-// Rows a lane group takes at once: four (their loads in flight together, weight and bias read once for them) where that still
-// leaves eight workgroups a CU, else one.
+// Rows a lane group takes at once: four (their loads in flight together) where that still leaves eight workgroups a CU, else one.
 template <int MODE, typename T, bool RAG, int LPR, int CH>
 static int launch_depth(const RowArgs& a, hipStream_t stream) {
     if constexpr (CH == 1) {

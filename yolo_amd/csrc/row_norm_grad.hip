@@ -138,23 +138,24 @@ __global__ __launch_bounds__(kThreads) void norm_grad_kernel(const GradArgs a) {
     }
 }
 
-// dw and db from the workgroups' partial sums: 16 columns a workgroup (of the 2 C), 16 lanes a column, each over every
-// sixteenth partial sum, then a tree over the 16.
-__global__ __launch_bounds__(kThreads) void norm_grad_sum_kernel(const float* part, int parts, int C, void* dgamma, void* dbeta,
-                                                                 int dtype) {
-    __shared__ float meet[16][17];
+// dw and db from the workgroups' partial sums: 16 columns a workgroup (of the 2 C), 64 lanes a column, each over every 64th
+// partial sum (eight loads in flight), then a tree over the 64.
+__global__ __launch_bounds__(1024) void norm_grad_sum_kernel(const float* part, int parts, int C, void* dgamma, void* dbeta,
+                                                             int dtype) {
+    __shared__ float meet[64][17];
     const int lc = threadIdx.x & 15, sl = threadIdx.x >> 4, col = blockIdx.x * 16 + lc;
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    float s = 0.f;
     if (col < 2 * C) {
         const float* p = part + col;
-        int k = sl;
-        for (; k + 48 < parts; k += 64)
+        for (int k = sl; k < parts; k += 64 * 8) {
+            float v[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[j] += p[(long long)(k + 16 * j) * 2 * C];
-        for (; k < parts; k += 16) s[0] += p[(long long)k * 2 * C];
+            for (int j = 0; j < 8; ++j) v[j] = k + 64 * j < parts ? p[(long long)(k + 64 * j) * 2 * C] : 0.f;
+            s += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+        }
     }
-    meet[sl][lc] = (s[0] + s[1]) + (s[2] + s[3]);
-    for (int h = 8; h >= 1; h >>= 1) {
+    meet[sl][lc] = s;
+    for (int h = 32; h >= 1; h >>= 1) {
         __syncthreads();
         if (sl < h) meet[sl][lc] += meet[sl + h][lc];
     }
@@ -169,11 +170,11 @@ __global__ __launch_bounds__(kThreads) void norm_grad_sum_kernel(const float* pa
     }
 }
 
-// Workgroups of the gradient kernel: by rows and channels alone, so that the size of the workspace is known without a GPU.
-// At least 8 rows a lane group (a partial sum costs as much as a row of fp32), at most 1024 workgroups (four a CU).
-static int grad_blocks(long long rows, int C) {
-    const int lpr = C > 2048 ? 256 : 64;
-    const long long per = (long long)(kThreads / lpr) * 8, n = (rows + per - 1) / per;
+// Workgroups of the gradient kernel: by rows alone, so that the size of the workspace is known without a GPU.  At least 8 rows
+// each (a partial sum, written and read, costs as much as three rows of bf16; with 2 rows each 3000 x 4096 took 48 us instead of
+// 31), at most 1024 workgroups (four a CU).
+static int grad_blocks(long long rows) {
+    const long long n = (rows + 7) / 8;
     return (int)(n < 1 ? 1 : n > 1024 ? 1024 : n);
 }
 
@@ -208,7 +209,7 @@ using namespace ydet::rows;
 
 extern "C" size_t ydet_layer_norm_backward_workspace_bytes(int64_t rows, int C) {
     if (rows < 0 || C <= 0 || C > kMaxC) return 0;
-    return (size_t)grad_blocks(rows, C) * 2 * C * sizeof(float);
+    return (size_t)grad_blocks(rows) * 2 * C * sizeof(float);
 }
 
 extern "C" int ydet_layer_norm_backward(const ydet_layer_norm_grad_desc* d, void* ws, size_t ws_bytes, void* stream) {
@@ -231,7 +232,7 @@ extern "C" int ydet_layer_norm_backward(const ydet_layer_norm_grad_desc* d, void
     a.dx = d->dx ? static_cast<char*>(d->dx) + d->dx_coff * es : nullptr;
     YDET_CHECK_ARG(((uintptr_t)a.x | (uintptr_t)a.dy | (uintptr_t)a.dx) % es == 0 && ((uintptr_t)d->dgamma | (uintptr_t)d->dbeta) % ps == 0,
                    "layer_norm_backward: misaligned tensor");
-    int blocks = grad_blocks(d->rows, d->C);
+    int blocks = grad_blocks(d->rows);
     if (params) {
         YDET_CHECK_ARG(ws && (uintptr_t)ws % 4 == 0, "layer_norm_backward: the weight's gradient needs a workspace");
         const size_t need = (size_t)blocks * 2 * d->C * sizeof(float);
@@ -251,7 +252,7 @@ extern "C" int ydet_layer_norm_backward(const ydet_layer_norm_grad_desc* d, void
         if (rc != YDET_OK) return rc;
     }
     if (params) {
-        hipLaunchKernelGGL(norm_grad_sum_kernel, dim3((unsigned)((2 * d->C + 15) / 16)), dim3(kThreads), 0, s, a.part,
+        hipLaunchKernelGGL(norm_grad_sum_kernel, dim3((unsigned)((2 * d->C + 15) / 16)), dim3(1024), 0, s, a.part,
                            d->rows > 0 ? blocks : 0, d->C, d->dgamma, d->dbeta, d->param_dtype);
         YDET_CHECK_LAUNCH("layer norm gradient of the weight");
     }
