@@ -42,7 +42,7 @@ typedef enum { YDET_RES_NONE = 0, YDET_RES_AFTER_ACT = 1, YDET_RES_BEFORE_ACT = 
 const char* ydet_last_error(void);
 /* ABI version of the library (bumped when a struct below changes); equals YDET_ABI_VERSION of the header it
  * was built from. */
-#define YDET_ABI_VERSION 16
+#define YDET_ABI_VERSION 17
 int ydet_abi_version(void);
 
 /* ------------------------------------------------------------------------------------------
@@ -577,7 +577,9 @@ typedef enum {
     YDET_OP_C3_TAIL = 12,   /* conv + conv2 + conv3: as ydet_c3_tail_fused */
     YDET_OP_RGB_CONV = 13,  /* conv: as ydet_rgb_conv3x3_nchw; iarg3 = image dtype */
     YDET_OP_FOCUS_PAIR = 14,/* conv + conv2: as ydet_focus_conv_pair_nchw; iarg3 = image dtype */
-    YDET_OP_RGB_PAIR = 15   /* conv + conv2: as ydet_rgb_conv_pair_nchw; iarg3 = image dtype */
+    YDET_OP_RGB_PAIR = 15,  /* conv + conv2: as ydet_rgb_conv_pair_nchw; iarg3 = image dtype */
+    YDET_OP_LAYER_NORM = 16,/* norm: as ydet_layer_norm */
+    YDET_OP_LINEAR_I8 = 17  /* rows + product + workspace: as ydet_linear_i8 */
 } ydet_op_kind;
 
 typedef struct {
@@ -588,6 +590,11 @@ typedef struct {
     ydet_head_desc head;   /* YDET_OP_HEAD_DECODE */
     ydet_conv_desc conv2;  /* YDET_OP_BOTTLENECK, YDET_OP_C3_TAIL: the 3x3 stage */
     ydet_conv_desc conv3;  /* YDET_OP_C3_TAIL: cv3 */
+    ydet_layer_norm_desc norm;    /* YDET_OP_LAYER_NORM */
+    ydet_quantize_desc rows;      /* YDET_OP_LINEAR_I8 */
+    ydet_matmul_i8_desc product;
+    void* workspace;
+    int64_t workspace_bytes;
 } ydet_op;
 
 int ydet_run_ops(const ydet_op* ops /* host */, int n_ops, void* stream);

@@ -9,7 +9,7 @@ import math
 import pytest
 import torch
 
-from yolo_amd import _ffi, ops
+from yolo_amd import _ffi, engine, ops
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -512,3 +512,162 @@ def test_refusals():
             (lambda: ops.LinearI8(q, s[:3]), ValueError), (lambda: ops.LinearI8.quantize(torch.randn(4, 4, 3, 3, device=DEV)), ValueError)):
         with pytest.raises(err):
             call()
+
+
+# ---- in the planner -----------------------------------------------------------------------------------------------------------
+@pytest.fixture
+def pointwise_int8():
+    engine.set_pointwise_int8(True)
+    try:
+        yield
+    finally:
+        engine.set_pointwise_int8(False)
+        engine.set_compute_dtype(None)
+
+
+def _slice(arena, t):
+    root, off = t.resolve()
+    return arena[root][..., off:off + t.C]
+
+
+def _overlap(a, b):
+    (ra, oa), (rb, ob) = a.resolve(), b.resolve()
+    return ra is rb and oa < ob + b.C and ob < oa + a.C
+
+
+def _intact(opslist, i):
+    """Whether the maps of op i still hold what it read and wrote: not external, not worked on in place by it or a later op."""
+    a = opslist[i][1]
+    mine = [t for t in (a["x"], a["y"], a["res"]) if t is not None]
+    return (not any(t.resolve()[0].external for t in mine) and not any(_overlap(t, a["y"]) for t in mine if t is not a["y"])
+            and not any(_overlap(t, w) for _, later in opslist[i + 1:] for w in (later.get("y"), later.get("y2")) if w is not None for t in mine))
+
+
+def _check_products(plan):
+    """Every 8-bit convolution of a plan that ran and whose maps are intact: its output equals linear_i8 of its input, bit for bit."""
+    seen = 0
+    for arena in plan.arenas:
+        for i, (kind, a) in enumerate(plan.g.ops):
+            if kind != "linear_i8" or not _intact(plan.g.ops, i):
+                continue
+            act = {_ffi.ACT_NONE: "none", _ffi.ACT_LEAKY: "leaky", _ffi.ACT_SILU: "silu"}[a["act"]]
+            res = None if a["res"] is None else _slice(arena, a["res"])
+            want = ops.linear_i8(_slice(arena, a["x"]), a["lin"], act, a["slope"], res, "before" if a["res_mode"] == _ffi.RES_BEFORE_ACT else "after",
+                                 BF16)
+            assert torch.equal(_slice(arena, a["y"]), want)
+            seen += 1
+    return seen
+
+
+def test_plan_layers_in_8_bits(pointwise_int8):
+    """1x1 layers with SiLU / leaky / no activation, residual after and before it, into and out of concat buffers, and a layer
+    norm between them; against the operators and against the bf16 plan."""
+    from yolo_amd.synthetic import init_deterministic
+    from yolo_amd.yolov5_official.modules import Conv
+
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.a, self.b, self.c = Conv(512, 512), Conv(512, 512), torch.nn.Conv2d(1024, 512, 1)
+            self.n, self.d = torch.nn.LayerNorm(1024), Conv(512, 1024, act=False)
+
+        def lower(self, g, x):
+            a = self.a.lower(g, x)
+            b = self.b.lower(g, a, res=x)
+            c = g.conv(g.cat([a, b]), self.c, act=_ffi.ACT_LEAKY, slope=0.1, res=x, res_mode=_ffi.RES_BEFORE_ACT)
+            return g.layer_norm(self.d.lower(g, c), self.n)
+
+        def forward(self, x):
+            a = self.a(x)
+            b = x + self.b(a)
+            c = torch.nn.functional.leaky_relu(self.c(torch.cat([a, b], 1)) + x, 0.1)
+            return self.n(self.d(c).permute(0, 2, 3, 1)).permute(0, 3, 1, 2)
+
+    net = Net()
+    init_deterministic(net, seed=3)
+    net = net.to(DEV).eval()
+    with torch.no_grad():
+        net.n.weight.uniform_(0.5, 1.5)
+        net.n.bias.normal_()
+    x = randn(gen(2), 2, 512, 13, 11)
+    outs = {}
+    for on in (True, False):
+        engine.set_pointwise_int8(on)
+        g = engine.Graph(DEV, "bf16")
+        g.to_nchw(net.lower(g, g.input_nchw(*x.shape)), "y")
+        plan = g.finalize()
+        outs[on] = plan.run(x)["y"].float()
+        kinds = [k for k, _ in g.ops]
+        assert kinds.count("linear_i8") == (4 if on else 0) and kinds.count("layernorm") == 1 and "copy" not in kinds
+        assert _check_products(plan) == (4 if on else 0)
+        (nk, na), = [(k, a) for k, a in g.ops if k == "layernorm"]
+        assert torch.equal(_slice(plan.arenas[0], na["y"]), ops.layer_norm(_slice(plan.arenas[0], na["x"]), net.n.weight, net.n.bias, net.n.eps))
+        assert torch.equal(plan.run(x)["y"].float(), outs[on])
+    with torch.no_grad():
+        ref = net(x)
+    # bf16: every stored value is off by up to 2^-8 of itself, five maps deep, and so are the weights; 8 bits add steps of amax / 127
+    # (amax about 4.5 sigma: 1 % of a row's norm) four times to rows and weights
+    rel = lambda a: float((a - ref).norm() / ref.norm())
+    assert rel(outs[False]) < 5 * 2 * 2.0 ** -8 and rel(outs[True]) < 4 * 2 * 0.0125 + 5 * 2 * 2.0 ** -8
+
+
+def test_plan_layer_norm_fp32_and_refusal():
+    g = engine.Graph(DEV, "fp32")
+    n = torch.nn.LayerNorm(24, elementwise_affine=False).to(DEV)
+    x = randn(gen(4), 3, 24, 5, 7)
+    t = g.input_nchw(*x.shape)
+    with pytest.raises(NotImplementedError):
+        g.layer_norm(t, torch.nn.LayerNorm(12))
+    g.to_nchw(g.layer_norm(t, n), "y")
+    y = g.finalize().run(x)["y"]
+    assert torch.equal(y, ops.layer_norm(x.permute(0, 2, 3, 1)).permute(0, 3, 1, 2))
+
+
+@pytest.mark.parametrize("tag,size,batch", [("v3spp", 128, 1), ("v4", 128, 2)])
+def test_detector_in_8_bits(pointwise_int8, tag, size, batch):
+    """A whole detector with its 1x1 layers in 8 bits: every product checked against the operator on the plan's own maps; switching
+    the option off again gives the bf16 result of before."""
+    from helpers import build_fa
+    from yolo_amd.synthetic import images
+    engine.set_compute_dtype("bf16")
+    net = build_fa(tag, size).to(DEV)
+    x = images(batch, size, seed=1).to(DEV)
+    engine.set_pointwise_int8(False)
+    with torch.no_grad():
+        before = net(x)
+        engine.set_pointwise_int8(True)
+        net(x)
+        plans = [p for p in net._plans().plans.values() if any(k == "linear_i8" for k, _ in p.g.ops)]
+        torch.cuda.synchronize()
+        assert len(plans) == 1 and _check_products(plans[0]) >= 5
+        engine.set_pointwise_int8(False)
+        after = net(x)
+    for a, b in zip(before, after):
+        assert (a == b).all()
+
+
+def test_plan_in_8_bits_replicas_and_graph(pointwise_int8):
+    """Two side-by-side launch lists have workspaces of their own; a plan captured into a graph replays like its eager run."""
+    from yolo_amd.synthetic import init_deterministic
+    from yolo_amd.yolov5_official.modules import Conv
+    net = torch.nn.Sequential(Conv(512, 1024), Conv(1024, 512))
+    init_deterministic(net, seed=3)
+    net = net.to(DEV).eval()
+    x = randn(gen(2), 16, 512, 9, 9)
+
+    def build(n):
+        g = engine.Graph(DEV, "bf16")
+        g.to_nchw(engine.lower_any(g, net, g.input_nchw(n, 512, 9, 9)), "y")
+        return g
+    one, two = build(16).finalize(), build(8).finalize(2)
+    assert len(two.i8_ws) == 2 and two.i8_ws[0].data_ptr() != two.i8_ws[1].data_ptr()
+    want = one.run(x)["y"]
+    for _ in range(3):
+        assert torch.equal(two.run(x)["y"], want)
+    assert _check_products(two) == 4
+    replay = engine.GraphReplay(lambda t: one.run(t)["y"])
+    for k in range(4):
+        xk = x * (k + 1)
+        want = one.run(xk)["y"].clone()
+        assert torch.equal(replay(xk), want)
+        torch.cuda.synchronize()

@@ -104,3 +104,32 @@ def test_cpu_tensors_are_refused():
                  lambda: ops.LinearI8(torch.zeros(2, 4, dtype=torch.int8), torch.ones(2))):
         with pytest.raises(RuntimeError):
             call()
+
+
+# ---- the planner's choice of 8-bit layers ---------------------------------------------------------------------------------------
+def test_which_layers_go_to_8_bits():
+    from yolo_amd import engine
+    assert engine._pointwise_int8 is False
+    pays = engine.pointwise_int8_pays
+    assert pays(361, 4096, 512) and pays(400, 512, 512) and pays(6400, 2048, 1024) and pays(25600, 512, 2048) and pays(102400, 256, 1024)
+    assert not pays(25600, 512, 512) and not pays(102400, 1024, 256) and not pays(409600, 128, 512) and not pays(400, 256, 256)
+    g = engine.Graph("cpu", "bf16")
+    x = g.input_nchw(1, 512, 20, 20)
+    conv = lambda i, o, k=1, s=1, **kw: torch.nn.Conv2d(i, o, k, s, k // 2, **kw)
+    g.conv(x, conv(512, 512))                                   # 1: taken
+    g.conv(x, conv(512, 512, 3))                                # not 1x1
+    g.conv(x, conv(512, 512, 1, 2))                             # strided
+    g.conv(x, conv(512, 512, groups=2))                         # grouped
+    g.conv(x, conv(512, 255))                                   # prediction layer: no whole pieces
+    g.conv(x, conv(512, 512), out_dtype=_ffi.F32)               # fp32 map
+    y = g.conv(x, conv(512, 64))                                # 7: taken
+    g.conv(y, conv(64, 64))                                     # short sums
+    g.conv(x, conv(512, 512), post=(torch.nn.BatchNorm2d(512), None, _ffi.ACT_LEAKY, 0.1))      # a second stage
+    g.conv(x, conv(512, 512), res=x, res_mode=_ffi.RES_AFTER_ACT)                               # 10: taken
+    assert g.pointwise_int8() == [1, 7, 10]
+    engine.set_pointwise_int8(True)
+    try:
+        plan = g.finalize()                                     # (no GPU here: nothing is replaced)
+    finally:
+        engine.set_pointwise_int8(False)
+    assert not any(k == "linear_i8" for k, _ in plan.g.ops) and plan.i8_ws == [None]

@@ -14,9 +14,10 @@ F32, BF16, U8 = 0, 1, 2   # U8: output dtype of ydet_preprocess_u8 only
 ACT_NONE, ACT_LEAKY, ACT_SILU = 0, 1, 2
 RES_NONE, RES_AFTER_ACT, RES_BEFORE_ACT = 0, 1, 2
 (OP_CONV, OP_MAXPOOL2, OP_MAXPOOL2S1, OP_SPP, OP_UPSAMPLE, OP_SPACE2DEPTH, OP_COPY, OP_NCHW2NHWC,
- OP_NHWC2NCHW, OP_FOCUS_CONV, OP_HEAD_DECODE, OP_BOTTLENECK, OP_C3_TAIL, OP_RGB_CONV, OP_FOCUS_PAIR, OP_RGB_PAIR) = range(16)
+ OP_NHWC2NCHW, OP_FOCUS_CONV, OP_HEAD_DECODE, OP_BOTTLENECK, OP_C3_TAIL, OP_RGB_CONV, OP_FOCUS_PAIR, OP_RGB_PAIR,
+ OP_LAYER_NORM, OP_LINEAR_I8) = range(18)
 MAX_ANCHORS = 8
-ABI_VERSION = 16   # YDET_ABI_VERSION of include/ydet.h these structs were written against
+ABI_VERSION = 17   # YDET_ABI_VERSION of include/ydet.h these structs were written against
 
 
 class ConvDesc(C.Structure):
@@ -115,6 +116,8 @@ class Op(C.Structure):
     _fields_ = [
         ("kind", C.c_int32), ("iarg", C.c_int32), ("iarg2", C.c_int32), ("iarg3", C.c_int32),
         ("conv", ConvDesc), ("slice", SliceDesc), ("head", HeadDesc), ("conv2", ConvDesc), ("conv3", ConvDesc),
+        ("norm", LayerNormDesc), ("rows", QuantizeDesc), ("product", MatmulI8Desc), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
     ]
 
 

@@ -536,23 +536,31 @@ extern "C" size_t ydet_linear_i8_workspace_bytes(int64_t rows, int K) {
     return (size_t)rows * ((K + 15) / 16 * 16) + (size_t)(rows + 3) / 4 * 16;
 }
 
-extern "C" int ydet_linear_i8(const ydet_quantize_desc* in, const ydet_matmul_i8_desc* product, void* workspace, size_t workspace_bytes,
-                              void* stream) {
-    clear_error();
+int ydet_launch_linear_i8(const ydet_quantize_desc* in, const ydet_matmul_i8_desc* product, void* ws, size_t ws_bytes, hipStream_t stream) {
     YDET_CHECK_ARG(in && product, "linear_i8: null descriptor");
     YDET_CHECK_ARG(in->rows == product->rows && in->C == product->K, "linear_i8: %lld x %d rows for a product of %lld x %d", (long long)in->rows,
                    in->C, (long long)product->rows, product->K);
+    YDET_CHECK_ARG(in->rows >= 0 && in->C > 0, "linear_i8: rows=%lld K=%d", (long long)in->rows, in->C);
     if (in->rows == 0) return YDET_OK;
     const size_t need = ydet_linear_i8_workspace_bytes(in->rows, in->C);
-    YDET_CHECK_ARG(need > 0 && workspace && (uintptr_t)workspace % 16 == 0, "linear_i8: needs a 16-byte aligned workspace");
-    if (workspace_bytes < need) return fail(YDET_ERR_WORKSPACE, "linear_i8: workspace %zu < %zu bytes", workspace_bytes, need);
+    YDET_CHECK_ARG(ws && (uintptr_t)ws % 16 == 0, "linear_i8: needs a 16-byte aligned workspace");
+    if (ws_bytes < need) return fail(YDET_ERR_WORKSPACE, "linear_i8: workspace %zu < %zu bytes", ws_bytes, need);
     ydet_quantize_desc q = *in;
     ydet_matmul_i8_desc p = *product;
     q.q_ld = p.x_ld = (in->C + 15) / 16 * 16, p.x_coff = 0;
-    p.x = q.q = static_cast<int8_t*>(workspace);
+    p.x = q.q = static_cast<int8_t*>(ws);
     p.x_scale = q.scale = reinterpret_cast<float*>(q.q + in->rows * q.q_ld);
-    const int rc = ydet_launch_quantize_rows(&q, as_stream(stream));
-    return rc != YDET_OK ? rc : ydet_launch_matmul_i8(&p, nullptr, 0, as_stream(stream));
+    i8::Args a;
+    bool wide_x;
+    int rc = fill_args(&p, a, wide_x);      // (nothing is launched for a product that would be refused)
+    if (rc == YDET_OK) rc = ydet_launch_quantize_rows(&q, stream);
+    return rc != YDET_OK ? rc : ydet_launch_matmul_i8(&p, nullptr, 0, stream);
+}
+
+extern "C" int ydet_linear_i8(const ydet_quantize_desc* in, const ydet_matmul_i8_desc* product, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+    clear_error();
+    return ydet_launch_linear_i8(in, product, workspace, workspace_bytes, as_stream(stream));
 }
 
 extern "C" int ydet_matmul_i8(const ydet_matmul_i8_desc* d, void* workspace, size_t workspace_bytes, void* stream) {

@@ -123,6 +123,9 @@ static int launch_op(const ydet_op& op, hipStream_t s) {
         case YDET_OP_RGB_CONV: return ydet_launch_rgb_conv(&op.conv, op.iarg3, s);
         case YDET_OP_HEAD_DECODE: return ydet_launch_head_decode(&op.conv, &op.head, s);
         case YDET_OP_BOTTLENECK: return ydet_launch_bottleneck(&op.conv, &op.conv2, nullptr, s);
+        case YDET_OP_LAYER_NORM: return ydet_launch_layer_norm(&op.norm, s);
+        case YDET_OP_LINEAR_I8:
+            return ydet_launch_linear_i8(&op.rows, &op.product, op.workspace, op.workspace_bytes > 0 ? (size_t)op.workspace_bytes : 0, s);
         case YDET_OP_C3_TAIL: return ydet_launch_bottleneck(&op.conv, &op.conv2, &op.conv3, s);
         case YDET_OP_MAXPOOL2:
         case YDET_OP_MAXPOOL2S1:

@@ -342,6 +342,18 @@ class Graph:
         self.ops.append((kind, dict(x=x, y=out, iarg=iarg)))
         return out
 
+    def layer_norm(self, x, norm, out=None):
+        """nn.LayerNorm over the channels of every pixel (what `x.permute(0, 2, 3, 1)` -> norm -> permute back computes)."""
+        if tuple(norm.normalized_shape) != (x.C,):
+            raise NotImplementedError(f"layer norm over {tuple(norm.normalized_shape)}: the lowering normalises the {x.C} channels")
+        if out is None:
+            out = self.new(x.N, x.H, x.W, x.C, dtype=x.dtype)
+        assert (out.N, out.H, out.W, out.C, out.dtype) == (x.N, x.H, x.W, x.C, x.dtype), "layer norm output shape mismatch"
+        w, b = (p if p is None else p.detach().to(device=self.device, dtype=torch.float32).contiguous() for p in (norm.weight, norm.bias))
+        self.keep.append((w, b))
+        self.ops.append(("layernorm", dict(x=x, y=out, w=w, b=b, eps=float(norm.eps))))
+        return out
+
     def maxpool2(self, x):
         return self._slice_op("maxpool2", x, self.new(x.N, x.H // 2, x.W // 2, x.C))
 
@@ -621,6 +633,33 @@ class Graph:
             del self.ops[j]
             self.ext_in = [i - 1 if i > j else i for i in self.ext_in]
 
+    # ---- 1x1 convolutions in 8-bit integers ---------------------------------------------------------------------------
+    def pointwise_int8(self):
+        """Indices of the convolutions that set_pointwise_int8 moves to 8 bits: 1x1 / stride 1, nothing fused in but bias,
+        activation and residual, whole 16-byte pieces of output, and a shape that gains (pointwise_int8_pays)."""
+        found = []
+        for i, (kind, a) in enumerate(self.ops):
+            if kind != "conv" or any(a.get(k) is not None for k in ("post", "y2", "up", "pre")):
+                continue
+            x, y, pc = a["x"], a["y"], a["pc"]
+            if (pc.plain and (pc.KH, pc.KW, a["stride"], a["pad"]) == (1, 1, 1, 0) and x.dtype == y.dtype == _ffi.BF16 and pc.Cout % 8 == 0
+                    and x.C <= 8192 and pointwise_int8_pays(x.N * x.H * x.W, x.C, pc.Cout)):
+                found.append(i)
+        return found
+
+    def lower_pointwise_int8(self):
+        """Replace those convolutions by quantisation of the pixels' rows + product in 8 bits.  The folded weights take one
+        scale per output channel, the pixels one each, found on the way."""
+        if not _pointwise_int8 or self.dt != _ffi.BF16 or self.device.type != "cuda":
+            return
+        from .ops import LinearI8
+        for i in self.pointwise_int8():
+            a = self.ops[i][1]
+            pc = a["pc"]
+            lin = LinearI8.quantize(pc.w[:pc.Cout, :a["x"].C].float(), pc.b[:pc.Cout])
+            self.keep.append(lin)
+            self.ops[i] = ("linear_i8", dict(a, lin=lin))
+
     # ---- finalize ------------------------------------------------------------------------------
     def finalize(self, replicas=1):
         return Plan(self, replicas)
@@ -643,6 +682,7 @@ class Plan:
         g.fuse_rgb_stem()
         g.fuse_rgb_pool()
         g.fuse_focus_pair()
+        g.lower_pointwise_int8()
         n = len(g.ops)
         self.patch_in = list(g.ext_in)  # op indices whose source is a caller-supplied NCHW input
         self.patch_out = []       # (op index, field, storage) of external NHWC buffers
@@ -686,6 +726,15 @@ class Plan:
                 for op, nb in zip(ops, need):
                     if nb > 0:
                         op.conv.splitk_ws, op.conv.splitk_ws_bytes = ws.data_ptr(), ws.numel()
+        # rows in 8 bits of the products (set_pointwise_int8): one workspace per launch list, likewise
+        self.i8_ws = []
+        for ops in self.op_lists:
+            need = [_ffi.lib().ydet_linear_i8_workspace_bytes(op.rows.rows, op.rows.C) if op.kind == _ffi.OP_LINEAR_I8 else 0 for op in ops]
+            ws = torch.empty(max(need), dtype=torch.uint8, device=g.device) if max(need, default=0) > 0 else None
+            self.i8_ws.append(ws)
+            for op, nb in zip(ops, need):
+                if nb > 0:
+                    op.workspace, op.workspace_bytes = ws.data_ptr(), ws.numel()
         self.ops = self.op_lists[0]
         # run() writes the caller's pointers into the shared launch records and then enqueues them: one host thread at a
         # time per plan (the enqueue copies the records into kernel arguments, so the lock ends with the call)
@@ -704,6 +753,16 @@ class Plan:
     def _fill(self, op, i, kind, a, arena, record, with_y=True):
         if kind == "conv":
             self._fill_conv(op, i, a, arena, record)
+        elif kind == "linear_i8":
+            self._fill_linear_i8(op, i, a, arena, record)
+        elif kind == "layernorm":
+            op.kind = _ffi.OP_LAYER_NORM
+            (rx, ox), (ry, oy) = a["x"].resolve(), a["y"].resolve()
+            x, nd = a["x"], op.norm
+            nd.x, nd.y = self._ptr(rx, arena, i, "nx", record), self._ptr(ry, arena, i, "ny", record)
+            nd.gamma, nd.beta = (p if p is None else p.data_ptr() for p in (a["w"], a["b"]))
+            nd.rows, nd.C, nd.x_ld, nd.x_coff, nd.y_ld, nd.y_coff = x.N * x.H * x.W, x.C, rx.ld, ox, ry.ld, oy
+            nd.dtype, nd.param_dtype, nd.eps = rx.dtype, _ffi.F32, a["eps"]
         elif kind == "bottleneck":
             assert not a["x"].resolve()[0].external and not a["y"].resolve()[0].external
             self._fill_conv(op, i, a["cv1"], arena, record)
@@ -782,6 +841,21 @@ class Plan:
             sl.x, sl.y = self._ptr(rx, arena, i, "x", record), self._ptr(ry, arena, i, "y", record)
             sl.N, sl.H, sl.W, sl.C = x.N, x.H, x.W, x.C
             sl.x_ld, sl.x_coff, sl.y_ld, sl.y_coff, sl.dtype = rx.ld, ox, ry.ld, oy, rx.dtype
+
+    def _fill_linear_i8(self, op, i, a, arena, record):
+        op.kind = _ffi.OP_LINEAR_I8
+        x, lin = a["x"], a["lin"]
+        (rx, ox), (ry, oy) = x.resolve(), a["y"].resolve()
+        r, p = op.rows, op.product
+        r.x, p.y = self._ptr(rx, arena, i, "qx", record), self._ptr(ry, arena, i, "qy", record)
+        r.rows, r.C, r.x_ld, r.x_coff, r.dtype = x.N * x.H * x.W, x.C, rx.ld, ox, rx.dtype
+        p.rows, p.K, p.N, p.kp, p.n_pad = r.rows, lin.K, lin.N, lin.kp, lin.n_pad
+        p.w, p.w_scale, p.bias = lin.w.data_ptr(), lin.scale.data_ptr(), lin.bias.data_ptr()
+        p.y_ld, p.y_coff, p.out_dtype, p.act, p.slope = ry.ld, oy, ry.dtype, a["act"], a["slope"]
+        if a["res"] is not None:
+            rr, orr = a["res"].resolve()
+            assert rr.dtype == ry.dtype
+            p.res, p.res_ld, p.res_coff, p.res_mode = self._ptr(rr, arena, i, "qres", record), rr.ld, orr, a["res_mode"]
 
     def _fill_conv(self, op, i, a, arena, record, d=None, skip_x=False):
         op.kind = _ffi.OP_CONV
@@ -887,6 +961,16 @@ class Plan:
                     op.conv.x = ptr
                 elif field == "cy":
                     op.conv.y = ptr
+                elif field == "qx":
+                    op.rows.x = ptr
+                elif field == "qy":
+                    op.product.y = ptr
+                elif field == "qres":
+                    op.product.res = ptr
+                elif field == "nx":
+                    op.norm.x = ptr
+                elif field == "ny":
+                    op.norm.y = ptr
                 elif field == "hz":
                     op.head.z = ptr
                 elif field == "hr":
@@ -927,6 +1011,7 @@ _fuse_focus_pair = True
 _fuse_rgb_pool = True
 _head_raw_compute = True
 _split_k = False
+_pointwise_int8 = False
 
 
 def set_focus_pair_fusion(flag):
@@ -950,6 +1035,24 @@ def set_split_k(flag):
     batch equals its own single-image run bit for bit."""
     global _split_k
     _split_k = bool(flag)
+
+
+def set_pointwise_int8(flag):
+    """Whether bf16 plans run 1x1 convolutions in 8-bit integers where that is faster (default off): the folded weights with
+    one scale per output channel, every pixel's channels with a scale of their own that is found when the layer runs (no
+    calibration).  A layer's output then differs by about 1 % of its norm; prediction layers stay as they are.  Whether a layer
+    is taken goes by its shape (pointwise_int8_pays), so an image's result may differ between batch sizes."""
+    global _pointwise_int8
+    _pointwise_int8 = bool(flag)
+
+
+def pointwise_int8_pays(rows, cin, cout):
+    """Quantisation + product against the bf16 kernels on MI355X, us: the pass that quantises costs the narrow layers of large
+    batches more than the product saves (25600 pixels 512 -> 512: 29 against 24, 102400 pixels 1024 -> 256: 115 against 81).  It
+    pays where few pixels meet a long sum (361 pixels 4096 -> 512: 16 against 42; 400 pixels 512 -> 512: 7.6 against 9.7; 6400
+    pixels 2048 -> 1024: 34 against 37) and where a layer widens (25600 pixels 512 -> 2048: 68 against 88, 102400 pixels 256 ->
+    1024: 97 against 104; but 409600 pixels 128 -> 512: 179 against 166)."""
+    return (rows <= 6400 and cin >= 512) or (cin >= 256 and cout >= 2 * cin)
 
 
 def set_head_raw_dtype(mode):
@@ -1110,6 +1213,12 @@ def _op_info(kind, a):
                     flops=flops,
                     bytes=nbytes,
                     shape=(x.N, x.H, x.W, x.C, pc.Cout, pc.KH, a["stride"]))
+    if kind == "linear_i8":
+        x, y, pc = a["x"], a["y"], a["pc"]
+        px = y.N * y.H * y.W
+        return dict(kind="conv", label="linear_i8", flops=2.0 * px * pc.Cout * pc.cin_real,
+                    bytes=px * x.C * esz(x) + px * pc.Cout * esz(y) * (1 if a["res"] is None else 2) + pc.Cout * x.C,
+                    shape=(x.N, x.H, x.W, x.C, pc.Cout, 1, 1))
     if kind == "c3tail":
         x, y = a["x"], a["y"]
         px = y.N * y.H * y.W
@@ -1184,7 +1293,8 @@ class PlanCache:
         # not share one, so the stream is part of the key (callers that pipeline batches over two streams get two plans)
         # the planner switches (fusions on / off, dtype of the raw head maps, batch split) shape the launch list: a
         # plan built under other settings is not reused
-        key = (key, _fuse_upsample, _fuse_followers, _fuse_focus_pair, _fuse_rgb_pool, _head_raw_compute, _batch_split, _split_k)
+        key = (key, _fuse_upsample, _fuse_followers, _fuse_focus_pair, _fuse_rgb_pool, _head_raw_compute, _batch_split, _split_k,
+               _pointwise_int8)
         if torch.cuda.is_available() and torch.cuda.is_initialized():
             key = (key, torch.cuda.current_stream().cuda_stream)
         p = self.plans.get(key)
