@@ -346,6 +346,32 @@ def test_matmul_i8_does_not_depend_on_the_batch(out):
         assert torch.equal(ops.matmul_i8(q[:n], s[:n], lin, act="silu", out_dtype=out), y[:n])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M,K,N", [(1, 1, 1), (1, 1024, 1024), (5, 77, 33), (16, 2048, 512), (17, 2049, 75), (100, 1000, 255), (400, 1024, 512),
+                                   (200, 100, 1000), (169, 384, 1536), (300, 1025, 256), (33, 8192, 64), (3000, 200, 130)])
+def test_linear_i8_is_quantisation_and_product(M, K, N, dtype):
+    """In one launch or two: the bits of quantize_rows followed by matmul_i8, rows without a scale and rows of zeros among them."""
+    g = gen(M + 3 * K + 7 * N)
+    x = (randn(g, M, K) * torch.exp(2 * randn(g, M, 1))).to(dtype)
+    x[M // 2] = 0
+    if M > 4:
+        x[1, K // 2], x[3, 0] = float("nan"), float("-inf")
+        x[4] = torch.where(torch.arange(K, device=DEV) % 2 == 0, 1.0, -0.5).to(dtype)        # every other value on a border
+    lin = ops.LinearI8.quantize(randn(g, N, K), randn(g, N))
+    wide = torch.zeros(M, K + 5, device=DEV, dtype=dtype)
+    wide[:, 3:K + 3] = x
+    for out in (F32, BF16):
+        res = randn(g, M, N, dtype=out)
+        q, s = ops.quantize_rows(x)
+        for kw in (dict(), dict(act="silu", res=res), dict(act="leaky", res=res, res_mode="before")):
+            want = ops.matmul_i8(q, s, lin, out_dtype=out, **kw)
+            for t in (x, wide[:, 3:K + 3]):
+                got = ops.linear_i8(t, lin, out_dtype=out, **kw)
+                assert torch.equal(got.nan_to_num(12345.0), want.nan_to_num(12345.0)) and torch.equal(got.isnan(), want.isnan())
+    if M > 4:
+        assert want[1].isnan().all() and want[3].isnan().all() and torch.isfinite(want[2]).all()
+
+
 def test_rows_at_any_distance_and_address():
     """Channel slices of wider maps, odd pitches and addresses, transposed and broadcast maps."""
     g = gen(21)

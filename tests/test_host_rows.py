@@ -53,6 +53,13 @@ def product(**kw):
     return _ffi.lib().ydet_matmul_i8(_ffi.MatmulI8Desc(**d), None, 0, None)
 
 
+def linear(ws=P, ws_bytes=1 << 40, rows=4, C_=64, **kw):
+    q = _ffi.QuantizeDesc(x=P, rows=rows, C=C_, x_ld=C_, dtype=1, param_dtype=0)
+    d = dict(w=P, w_scale=P, bias=P, y=P, rows=4, K=64, N=32, kp=64, n_pad=128, y_ld=32, out_dtype=1)
+    d.update(kw)
+    return _ffi.lib().ydet_linear_i8(q, _ffi.MatmulI8Desc(**d), ws, ws_bytes, None)
+
+
 ARG, WS = -1, -3
 
 
@@ -72,7 +79,10 @@ ARG, WS = -1, -3
     (product, dict(n_pad=64), "padded"), (product, dict(N=129, y_ld=160), "padded"), (product, dict(x_ld=63), "slice"), (product, dict(y_coff=1), "slice"),
     (product, dict(x_ld=(1 << 23) + 16), "x_ld"), (product, dict(out_dtype=2), "out_dtype"), (product, dict(act=3), "act"), (product, dict(res_mode=3), "act"),
     (product, dict(w=P + 8), "alignment"), (product, dict(w_scale=P + 4), "alignment"), (product, dict(y=P + 1), "misaligned"),
-    (product, dict(rows=(1 << 31) - 1), "rows")])
+    (product, dict(rows=(1 << 31) - 1), "rows"),
+    (linear, dict(rows=5), "product of"), (linear, dict(C_=65), "product of"), (linear, dict(w=None), "null"), (linear, dict(N=200, y_ld=200), "padded"),
+    (linear, dict(rows=1 << 20, C_=8193, K=8193, kp=8256), "product of"), (linear, dict(C_=8193, K=8193, kp=8256), "K="),
+    (linear, dict(rows=1 << 16, ws=None, **{"N": 32}), "product of")])
 def test_bad_arguments(call, kw, text):
     assert call(**kw) == ARG
     assert text in _ffi.lib().ydet_last_error().decode()
@@ -87,6 +97,28 @@ def test_workspace():
         assert sizes == sorted(sizes) and sizes[-1] <= 1024 * 2 * C_ * 4
     assert grad(ws_bytes=size(4, 32) - 4) == WS
     assert "workspace" in _ffi.lib().ydet_last_error().decode()
+
+
+def test_linear_workspace():
+    lib = _ffi.lib()
+
+    def sizes(rows, K, N, **kw):
+        q = _ffi.QuantizeDesc(x=P, rows=rows, C=K, x_ld=K, dtype=1, **kw)
+        kp, n_pad = (K + 63) // 64 * 64, (N + 127) // 128 * 128
+        d = _ffi.MatmulI8Desc(w=P, w_scale=P, y=P, rows=rows, K=K, N=N, kp=kp, n_pad=n_pad, y_ld=N, out_dtype=1)
+        return q, d, lib.ydet_linear_i8_workspace_bytes(q, d)
+    assert sizes(1, 1024, 1024)[2] == 0 and sizes(100, 2048, 512)[2] == 0           # one launch
+    assert sizes(100, 2049, 512)[2] == 100 * 2064 + 100 * 4 and sizes(400, 1024, 512)[2] == 400 * 1028 and sizes(25601, 500, 64)[2] == 25601 * 512 + 25604 * 4
+    q, d, n = sizes(25600, 500, 64)
+    assert lib.ydet_linear_i8(q, d, P, n - 1, None) == WS and "workspace" in lib.ydet_last_error().decode()
+    assert lib.ydet_linear_i8(q, d, None, n, None) == ARG
+    assert lib.ydet_linear_i8(q, d, P + 8, n, None) == ARG
+    assert sizes(4, 8193, 8)[2] == 0 and sizes(0, 64, 64)[2] == 0
+    # rows of x at odd addresses need a copy where they are many
+    rows = lambda n, ld: _ffi.MatmulI8Desc(x=P, x_scale=P, w=P, w_scale=P, y=P, rows=n, K=77, N=64, kp=128, n_pad=128, x_ld=ld, y_ld=64, out_dtype=1)
+    size = lib.ydet_matmul_i8_workspace_bytes
+    assert size(rows(100, 77)) == 0 and size(rows(50000, 80)) == 0 and size(rows(50000, 77)) == 50000 * 80 and size(rows(-1, 77)) == 0
+    assert lib.ydet_matmul_i8(rows(50000, 77), None, 0, None) == WS and lib.ydet_matmul_i8(rows(50000, 77), P + 4, 1 << 30, None) == ARG
 
 
 def test_nothing_to_do_is_no_error():

@@ -176,7 +176,7 @@ SYMBOLS = {
     "ydet_layer_norm_backward_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int]),
     "ydet_layer_norm_backward": (C.c_int, [C.POINTER(LayerNormGradDesc), C.c_void_p, C.c_size_t, C.c_void_p]),
     "ydet_quantize_rows_i8": (C.c_int, [C.POINTER(QuantizeDesc), C.c_void_p]),
-    "ydet_linear_i8_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int]),
+    "ydet_linear_i8_workspace_bytes": (C.c_size_t, [C.POINTER(QuantizeDesc), C.POINTER(MatmulI8Desc)]),
     "ydet_linear_i8": (C.c_int, [C.POINTER(QuantizeDesc), C.POINTER(MatmulI8Desc), C.c_void_p, C.c_size_t, C.c_void_p]),
     "ydet_matmul_i8_workspace_bytes": (C.c_size_t, [C.POINTER(MatmulI8Desc)]),
     "ydet_matmul_i8": (C.c_int, [C.POINTER(MatmulI8Desc), C.c_void_p, C.c_size_t, C.c_void_p]),

@@ -8,6 +8,7 @@
 // MFMA row, pixels on its column, and weight rows are fetched in an order that leaves a lane with whole runs of
 // consecutive channels of one pixel, which it finishes and stores in 16-byte pieces.
 #include "conv_common.h"
+#include "rows_common.h"
 
 namespace ydet {
 namespace i8 {
@@ -332,6 +333,42 @@ __device__ __forceinline__ i32x4 load_k16(const char* p, long long left) {
     return v;
 }
 
+// The waves' sums meet in LDS; wave j finishes pixel fragment j (xs: the scales of the lane's pixel in every fragment).
+template <typename OUT, int FN, int FM, int NW>
+__device__ __forceinline__ void finish_few(const Args& a, const i32x4 (&acc)[FN][FM], const float (&xs)[FM], i32x4 (*meet)[FN * FM][64], int n0,
+                                           int m0) {
+    static_assert(FM <= NW, "a wave for every pixel fragment");
+    using R = Run<OUT, FN>;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, p = lane & 15;
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j) meet[wave][j * FN + i][lane] = acc[i][j];
+    __syncthreads();
+    float x = xs[0];
+#pragma unroll
+    for (int j = 1; j < FM; ++j) x = wave == j ? xs[j] : x;
+    if (wave >= FM) return;
+    const int j = wave, m = m0 + j * 16 + p, n = n0 + q * R::PE;
+    int v[4 * FN];
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+        i32x4 s = meet[0][j * FN + i][lane];
+#pragma unroll
+        for (int k = 1; k < NW; ++k) s += meet[k][j * FN + i][lane];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i * 4 + e] = s[e];
+    }
+    float ws[4 * FN], bias[4 * FN];
+    load_channels<R>(a.ws + n, a.bias ? a.bias + n : nullptr, ws, bias);
+    with_mode(a, [&](auto mode) {
+        using M = decltype(mode);
+        R run;
+        run.template load_residual<M>(a, m, n);
+        run.template store<M>(a, m, n, x, v, ws, bias);
+    });
+}
+
 template <typename OUT, int FN, int FM, int NW, bool ANY>
 __global__ __launch_bounds__(64 * NW) void few_rows_kernel(const Args a) {
     constexpr int AHEAD = 4;        // steps of K whose loads are in flight
@@ -375,31 +412,83 @@ __global__ __launch_bounds__(64 * NW) void few_rows_kernel(const Args a) {
 #pragma unroll
                 for (int j = 0; j < FM; ++j) acc[i][j] = mma(fa[u][i], fb[u][j], acc[i][j]);
     }
+    float xs[FM];
 #pragma unroll
-    for (int i = 0; i < FN; ++i)
+    for (int j = 0; j < FM; ++j) xs[j] = a.xs[m0 + j * 16 + p < a.M ? m0 + j * 16 + p : a.M - 1];
+    finish_few<OUT, FN, FM, NW>(a, acc, xs, meet, n0, m0);
+}
+
+// The same from floating rows, 16 x 16 outputs a workgroup: its waves first find the rows' largest values together (their own K in
+// registers, so the rows are read once), then each quantises what it holds.  K up to 2048.  One launch instead of two at the
+// same time on the GPU (1 x 1024 -> 1024: 5.5 us against 5.8, 100 x 1024 -> 512: 7.4 against 6.9), which is less than the host's
+// time for a launch and a workspace.
+template <typename OUT, typename T, bool RAG>
+__global__ __launch_bounds__(512) void few_float_rows_kernel(const Args a) {
+    using namespace rows;
+    constexpr int NW = 8, AHEAD = 4, VEC = 16 / (int)sizeof(T), NV = 16 / VEC;
+    using P = Piece<T, VEC, true>;
+    using R = Run<OUT, 1>;
+    __shared__ __attribute__((aligned(16))) i32x4 meet[NW][1][64];
+    __shared__ unsigned tops[NW][16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, p = lane & 15;
+    const unsigned t = xcd_remap(blockIdx.x, gridDim.x);
+    const int n0 = (int)(t % (unsigned)a.tiles_n) * 16, m0 = (int)(t / (unsigned)a.tiles_n) * 16;
+    const int steps = a.kp / 64, m = m0 + p < a.M ? m0 + p : a.M - 1;
+    // Every load is made, pieces behind K from a page of zeros, so that all are in flight together.  RAG: the piece that holds the row's
+    // end also holds what follows it, cleared below; behind the last row it is read value by value.
+    typename P::type raw[AHEAD][NV];
+    i32x4 fa[AHEAD];
+    const T* px = reinterpret_cast<const T*>(a.x) + m * a.x_ld;
+    const char* pw = a.w + (long long)(n0 + channel_of<R::PE>(0, p >> 2, p & 3)) * a.kp + q * 16;
+    const long long left = (a.M - 1 - m) * a.x_ld + a.K;         // values from the row's first one to the end of all rows
 #pragma unroll
-        for (int j = 0; j < FM; ++j) meet[wave][j * FN + i][lane] = acc[i][j];
-    __syncthreads();
-    for (int j = wave; j < FM; j += NW) {
-        int v[4 * FN];
+    for (int u = 0; u < AHEAD; ++u) {
+        const int s = wave + u * NW;
 #pragma unroll
-        for (int i = 0; i < FN; ++i) {
-            i32x4 s = meet[0][j * FN + i][lane];
-#pragma unroll
-            for (int k = 1; k < NW; ++k) s += meet[k][j * FN + i][lane];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[i * 4 + e] = s[e];
+        for (int i = 0; i < NV; ++i) {
+            const int k = s * 64 + q * 16 + i * VEC;
+            const T* from = k < a.K && (!RAG || k + VEC <= left) ? px + k : reinterpret_cast<const T*>(conv::g_zero_chunk);
+            raw[u][i] = *reinterpret_cast<const typename P::loose*>(from);
         }
-        const int m = m0 + j * 16 + p, n = n0 + q * R::PE;
-        float ws[4 * FN], bias[4 * FN];
-        load_channels<R>(a.ws + n, a.bias ? a.bias + n : nullptr, ws, bias);
-        with_mode(a, [&](auto mode) {
-            using M = decltype(mode);
-            R run;
-            run.template load_residual<M>(a, m, n);
-            run.template store<M>(a, m, n, m < a.M ? a.xs[m] : 0.f, v, ws, bias);
-        });
+        fa[u] = *reinterpret_cast<const i32x4*>(s < steps ? pw + s * 64 : reinterpret_cast<const char*>(conv::g_zero_chunk));
     }
+    unsigned top = 0;
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int k = (wave + u * NW) * 64 + q * 16 + i * VEC;
+            if (RAG && k < a.K && k + VEC > left) raw[u][i] = P::load(px + k, (int)(left - k));
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                if (RAG) raw[u][i][e] = k + e < a.K ? raw[u][i][e] : (T)0.f;
+                top = MaxU{}(top, __float_as_uint((float)raw[u][i][e]) & 0x7fffffffu);
+            }
+        }
+    // the four lane groups hold the row's other columns
+    const auto r16 = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+    top = MaxU{}(r16[0], r16[1]);
+    const auto r32 = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+    top = MaxU{}(r32[0], r32[1]);
+    if (q == 0) tops[wave][p] = top;
+    __syncthreads();
+    top = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) top = MaxU{}(top, tops[w][p]);
+    const RowScale rs = row_scale(top);
+    i32x4 acc[1][1] = {{i32x4{0, 0, 0, 0}}};
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+        if (wave + u * NW >= steps) break;
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = rs.some ? (float)raw[u][i / VEC][i % VEC] : 0.f;
+        unsigned d[4];
+        quantise_pack(v, rs.s, rs.inv, d);
+        acc[0][0] = mma(fa[u], i32x4{(int)d[0], (int)d[1], (int)d[2], (int)d[3]}, acc[0][0]);
+    }
+    const float xs[1] = {rs.given};
+    finish_few<OUT, 1, 1, NW>(a, acc, xs, meet, n0, m0);
 }
 
 template <typename OUT, int BN, int BM, int WAVES_N, int WAVES_M, int NST = 2>
@@ -424,6 +513,15 @@ static int launch_few(Args a, hipStream_t stream) {
     YDET_CHECK_ARG(blocks * 64 * NW <= UINT32_MAX, "matmul_i8: %d rows x %d channels are too many tiles", a.M, a.N);
     hipLaunchKernelGGL((few_rows_kernel<OUT, FN, FM, NW, ANY>), dim3((unsigned)blocks), dim3(64 * NW), 0, stream, a);
     YDET_CHECK_LAUNCH("matmul_i8 (few rows)");
+    return YDET_OK;
+}
+
+template <typename OUT, typename T, bool RAG>
+static int launch_few_float(Args a, hipStream_t stream) {
+    a.tiles_n = (a.N + 15) / 16;
+    const long long blocks = (long long)a.tiles_n * ((a.M + 15) / 16);      // (one a CU at most)
+    hipLaunchKernelGGL((few_float_rows_kernel<OUT, T, RAG>), dim3((unsigned)blocks), dim3(512), 0, stream, a);
+    YDET_CHECK_LAUNCH("linear_i8 (few rows)");
     return YDET_OK;
 }
 
@@ -453,6 +551,15 @@ static long long tiles(const Args& a, int bn, int bm) { return (long long)((a.N 
 static int direct_size(const Args& a) {
     const int cus = current_device_info().cus;
     return tiles(a, 16, 16) <= 2 * cus ? 16 : tiles(a, 32, 32) <= cus ? 32 : 0;
+}
+
+// Whether floating rows are quantised by the product's own kernel: K fits its registers and there is at most a workgroup a CU (400 x
+// 100 -> 255, 400 workgroups, took 7.2 us, the two launches 5.6; a form for 32 x 32 outputs 12.3 us for 400 x 1024 -> 512, the two
+// launches 8.1: every workgroup quantises).
+static bool fuses(const Args& a) { return a.K <= 2048 && tiles(a, 16, 16) <= current_device_info().cus; }
+template <typename OUT, typename T>
+static int launch_fused(const Args& a, hipStream_t stream) {
+    return a.K % (16 / (int)sizeof(T)) ? launch_few_float<OUT, T, true>(a, stream) : launch_few_float<OUT, T, false>(a, stream);
 }
 
 template <typename OUT>
@@ -531,29 +638,53 @@ extern "C" size_t ydet_matmul_i8_workspace_bytes(const ydet_matmul_i8_desc* d) {
     return aligned_bytes(a);
 }
 
-extern "C" size_t ydet_linear_i8_workspace_bytes(int64_t rows, int K) {
-    if (rows < 0 || K <= 0) return 0;
-    return (size_t)rows * ((K + 15) / 16 * 16) + (size_t)(rows + 3) / 4 * 16;
-}
-
-int ydet_launch_linear_i8(const ydet_quantize_desc* in, const ydet_matmul_i8_desc* product, void* ws, size_t ws_bytes, hipStream_t stream) {
+// Checks the pair and fills the product's arguments as for rows in a workspace at `at` (any aligned address, to ask).
+static int fill_linear(const ydet_quantize_desc* in, const ydet_matmul_i8_desc* product, void* at, ydet_quantize_desc& q, ydet_matmul_i8_desc& p,
+                       i8::Args& a) {
     YDET_CHECK_ARG(in && product, "linear_i8: null descriptor");
     YDET_CHECK_ARG(in->rows == product->rows && in->C == product->K, "linear_i8: %lld x %d rows for a product of %lld x %d", (long long)in->rows,
                    in->C, (long long)product->rows, product->K);
-    YDET_CHECK_ARG(in->rows >= 0 && in->C > 0, "linear_i8: rows=%lld K=%d", (long long)in->rows, in->C);
-    if (in->rows == 0) return YDET_OK;
-    const size_t need = ydet_linear_i8_workspace_bytes(in->rows, in->C);
-    YDET_CHECK_ARG(ws && (uintptr_t)ws % 16 == 0, "linear_i8: needs a 16-byte aligned workspace");
-    if (ws_bytes < need) return fail(YDET_ERR_WORKSPACE, "linear_i8: workspace %zu < %zu bytes", ws_bytes, need);
-    ydet_quantize_desc q = *in;
-    ydet_matmul_i8_desc p = *product;
+    YDET_CHECK_ARG(in->rows >= 0 && in->rows <= INT32_MAX && in->C > 0 && in->C <= rows::kMaxC, "linear_i8: rows=%lld K=%d (K 1..%d)",
+                   (long long)in->rows, in->C, rows::kMaxC);
+    q = *in;
+    p = *product;
     q.q_ld = p.x_ld = (in->C + 15) / 16 * 16, p.x_coff = 0;
-    p.x = q.q = static_cast<int8_t*>(ws);
+    p.x = q.q = static_cast<int8_t*>(at);
     p.x_scale = q.scale = reinterpret_cast<float*>(q.q + in->rows * q.q_ld);
-    i8::Args a;
     bool wide_x;
-    int rc = fill_args(&p, a, wide_x);      // (nothing is launched for a product that would be refused)
-    if (rc == YDET_OK) rc = ydet_launch_quantize_rows(&q, stream);
+    return fill_args(&p, a, wide_x);
+}
+
+static bool fused(const ydet_quantize_desc& q, const i8::Args& a) { return !q.normalize && i8::fuses(a); }
+
+static size_t linear_bytes(const ydet_quantize_desc& q) { return (size_t)q.rows * q.q_ld + (size_t)(q.rows + 3) / 4 * 16; }
+
+extern "C" size_t ydet_linear_i8_workspace_bytes(const ydet_quantize_desc* in, const ydet_matmul_i8_desc* product) {
+    clear_error();
+    ydet_quantize_desc q;
+    ydet_matmul_i8_desc p;
+    i8::Args a;
+    if (fill_linear(in, product, reinterpret_cast<void*>(256), q, p, a) != YDET_OK || q.rows == 0 || fused(q, a)) return 0;
+    return linear_bytes(q);
+}
+
+int ydet_launch_linear_i8(const ydet_quantize_desc* in, const ydet_matmul_i8_desc* product, void* ws, size_t ws_bytes, hipStream_t stream) {
+    ydet_quantize_desc q;
+    ydet_matmul_i8_desc p;
+    i8::Args a;
+    int rc = fill_linear(in, product, ws ? ws : reinterpret_cast<void*>(256), q, p, a);
+    if (rc != YDET_OK || q.rows == 0) return rc;
+    if (fused(q, a)) {
+        rc = ydet_check_quantize_rows(&q);
+        if (rc != YDET_OK) return rc;
+        a.x = static_cast<const char*>(q.x) + q.x_coff * dtype_size(q.dtype), a.x_ld = q.x_ld, a.xs = nullptr;
+        if (q.dtype == YDET_BF16)
+            return p.out_dtype == YDET_BF16 ? i8::launch_fused<__bf16, __bf16>(a, stream) : i8::launch_fused<float, __bf16>(a, stream);
+        return p.out_dtype == YDET_BF16 ? i8::launch_fused<__bf16, float>(a, stream) : i8::launch_fused<float, float>(a, stream);
+    }
+    YDET_CHECK_ARG(ws && (uintptr_t)ws % 16 == 0, "linear_i8: needs a 16-byte aligned workspace");
+    if (ws_bytes < linear_bytes(q)) return fail(YDET_ERR_WORKSPACE, "linear_i8: workspace %zu < %zu bytes", ws_bytes, linear_bytes(q));
+    rc = ydet_launch_quantize_rows(&q, stream);
     return rc != YDET_OK ? rc : ydet_launch_matmul_i8(&p, nullptr, 0, stream);
 }
 

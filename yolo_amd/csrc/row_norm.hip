@@ -31,25 +31,6 @@ struct RowArgs {
 
 enum { kNorm = 1, kQuant = 2 };
 
-// a / b rounded once, with y the nearest number to 1 / b.  Markstein's step: q = a y, then q + (a - b q) y rounded once is the nearest
-// number to the quotient, as long as the remainder is exact, which tiny a do not allow.
-__device__ __forceinline__ float quotient(float a, float b, float y) {
-    const float q = a * y;
-    return fmaf(fmaf(-b, q, a), y, q);
-}
-
-// Nearest integer to v / s (ties to even), exactly, as a float's bits whose low byte is the integer.  The product with 1 / s
-// is within 3e-5 of the quotient, so rounding it (adding 1.5 * 2^23 leaves the integer in the low bits) is right unless it
-// lies that close to a border; there the remainder decides, which the fused multiply-add gives without error: near a
-// border |v - r s| is about s / 2 and a multiple of s's last place.
-__device__ __forceinline__ unsigned quantise_exact(float v, float s, float inv) {
-    constexpr float kMagic = 12582912.f;
-    float r = (v * inv + kMagic) - kMagic;
-    const float d = fmaf(-r, s, v), d2 = 2.f * fabsf(d);
-    if (d2 > s || (d2 == s && ((int)r & 1))) r += copysignf(1.f, d);
-    return __float_as_uint(r + kMagic);
-}
-
 template <int MODE, typename T, bool RAG, int LPR, int CH, int RPT>
 __global__ __launch_bounds__(kThreads) void row_norm_kernel(const RowArgs a) {
     constexpr int VEC = 16 / (int)sizeof(T);
@@ -130,49 +111,27 @@ __global__ __launch_bounds__(kThreads) void row_norm_kernel(const RowArgs a) {
                     }
                 }
             } else {
-                // largest magnitude by its bits: a NaN is above an infinity, and that above every number.  (Lanes and pieces
-                // behind the row's end hold zeros.)
+                // (lanes and pieces behind the row's end hold zeros)
                 unsigned top = 0;
 #pragma unroll
                 for (int i = 0; i < CH * VEC; ++i) {
                     const unsigned u = __float_as_uint(v[i]) & 0x7fffffffu;
                     top = u > top ? u : top;
                 }
-                top = group_reduce<LPR>(top, MaxU{}, red, slot);
-                const float amax = __uint_as_float(top);
-                const bool bad = top >= 0x7f800000u;                 // the row has no scale: NaN, and zeros
-                const bool some = !bad && amax >= 127.f * 1.17549435e-38f;   // smaller rows count as zero: s stays a normal number
-                const float s = !some ? 1.f : amax < 1e-25f ? amax / 127.f : quotient(amax, 127.f, 1.f / 127.f), inv = __builtin_amdgcn_rcpf(s);
-                if (live && l == 0) a.scale[row] = some ? s : bad ? __uint_as_float(0x7fc00000u) : 0.f;
-                unsigned m[CH * VEC];
-                float near = 0.f;
+                const RowScale rs = row_scale(group_reduce<LPR>(top, MaxU{}, red, slot));
+                if (live && l == 0) a.scale[row] = rs.given;
 #pragma unroll
-                for (int i = 0; i < CH * VEC; ++i) {
-                    constexpr float kMagic = 12582912.f;
-                    v[i] = some ? v[i] : 0.f;
-                    const float t = v[i] * inv, k = t + kMagic;
-                    near = fmaxf(near, fabsf(t - (k - kMagic)));
-                    m[i] = __float_as_uint(k);
-                }
-                if (near > 0.4999f) {
-#pragma unroll
-                    for (int i = 0; i < CH * VEC; ++i) m[i] = quantise_exact(v[i], s, inv);
-                }
+                for (int i = 0; i < CH * VEC; ++i) v[i] = rs.some ? v[i] : 0.f;
+                unsigned d[CH * VEC / 4];
+                quantise_pack(v, rs.s, rs.inv, d);
                 if (live) {
                     char* yr = a.y + row * a.y_ld;
 #pragma unroll
                     for (int c = 0; c < CH; ++c) {
                         const int col = (c * LPR + l) * VEC;
                         if (col < a.cw) {
-                            unsigned d[VEC / 4];
-#pragma unroll
-                            for (int j = 0; j < VEC / 4; ++j) {
-                                const unsigned lo = __builtin_amdgcn_perm(m[c * VEC + 4 * j + 1], m[c * VEC + 4 * j], 0x0c0c0400u);
-                                const unsigned hi = __builtin_amdgcn_perm(m[c * VEC + 4 * j + 3], m[c * VEC + 4 * j + 2], 0x0c0c0400u);
-                                d[j] = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
-                            }
-                            if constexpr (VEC == 8) *reinterpret_cast<uint2*>(yr + col) = make_uint2(d[0], d[1]);
-                            else *reinterpret_cast<unsigned*>(yr + col) = d[0];
+                            if constexpr (VEC == 8) *reinterpret_cast<uint2*>(yr + col) = make_uint2(d[2 * c], d[2 * c + 1]);
+                            else *reinterpret_cast<unsigned*>(yr + col) = d[c];
                         }
                     }
                 }
@@ -253,7 +212,8 @@ int ydet_launch_layer_norm(const ydet_layer_norm_desc* d, hipStream_t stream) {
     return launch_mode<kNorm>(a, d->dtype, stream);
 }
 
-int ydet_launch_quantize_rows(const ydet_quantize_desc* d, hipStream_t stream) {
+// What ydet_quantize_rows_i8 asks of its arguments.
+int ydet_check_quantize_rows(const ydet_quantize_desc* d) {
     YDET_CHECK_ARG(d, "quantize_rows: null descriptor");
     YDET_CHECK_ARG(d->rows >= 0 && d->rows <= INT32_MAX && d->C > 0 && d->C <= kMaxC, "quantize_rows: rows=%lld C=%d (C 1..%d)",
                    (long long)d->rows, d->C, kMaxC);
@@ -264,13 +224,19 @@ int ydet_launch_quantize_rows(const ydet_quantize_desc* d, hipStream_t stream) {
     YDET_CHECK_ARG(d->q_ld >= cw && d->q_ld % 16 == 0, "quantize_rows: rows of %d channels need q_ld >= %d, a multiple of 16 (got %d)", d->C,
                    cw, d->q_ld);
     YDET_CHECK_ARG(!d->normalize || d->eps >= 0.f, "quantize_rows: eps=%g", (double)d->eps);
-    if (d->rows == 0) return YDET_OK;
-    YDET_CHECK_ARG(d->x && d->q && d->scale, "quantize_rows: null pointer");
+    YDET_CHECK_ARG(d->rows == 0 || (d->x && d->q && d->scale), "quantize_rows: null pointer");
     const size_t es = dtype_size(d->dtype);
+    YDET_CHECK_ARG((uintptr_t)d->x % es == 0 && (uintptr_t)d->q % 16 == 0, "quantize_rows: misaligned tensor");
+    return YDET_OK;
+}
+
+int ydet_launch_quantize_rows(const ydet_quantize_desc* d, hipStream_t stream) {
+    const int rc = ydet_check_quantize_rows(d);
+    if (rc != YDET_OK || d->rows == 0) return rc;
     RowArgs a{};
-    a.x = static_cast<const char*>(d->x) + d->x_coff * es;
+    a.x = static_cast<const char*>(d->x) + d->x_coff * dtype_size(d->dtype);
     a.y = reinterpret_cast<char*>(d->q);
-    YDET_CHECK_ARG((uintptr_t)a.x % es == 0 && (uintptr_t)a.y % 16 == 0, "quantize_rows: misaligned tensor");
+    const int cw = (d->C + 15) / 16 * 16;
     a.scale = d->scale, a.rows = d->rows, a.C = d->C, a.cw = cw, a.x_ld = d->x_ld, a.y_ld = d->q_ld;
     a.gamma = static_cast<const char*>(d->gamma), a.beta = static_cast<const char*>(d->beta);
     a.param_dtype = d->param_dtype, a.eps = d->eps, a.inv_c = 1.f / (float)d->C;

@@ -82,6 +82,67 @@ __device__ __forceinline__ float group_sum(float v, unsigned (&red)[2][4], int& 
     return __uint_as_float(group_reduce<LPR>(__float_as_uint(v), AddF{}, red, slot));
 }
 
+// a / b rounded once, with y the nearest number to 1 / b.  Markstein's step: q = a y, then q + (a - b q) y rounded once is the nearest
+// number to the quotient, as long as the remainder is exact, which tiny a do not allow.
+__device__ __forceinline__ float quotient(float a, float b, float y) {
+    const float q = a * y;
+    return fmaf(fmaf(-b, q, a), y, q);
+}
+
+// Nearest integer to v / s (ties to even), exactly, as a float's bits whose low byte is the integer.  The product with 1 / s
+// is within 3e-5 of the quotient, so rounding it (adding 1.5 * 2^23 leaves the integer in the low bits) is right unless it
+// lies that close to a border; there the remainder decides, which the fused multiply-add gives without error: near a
+// border |v - r s| is about s / 2 and a multiple of s's last place.
+__device__ __forceinline__ unsigned quantise_exact(float v, float s, float inv) {
+    constexpr float kMagic = 12582912.f;
+    float r = (v * inv + kMagic) - kMagic;
+    const float d = fmaf(-r, s, v), d2 = 2.f * fabsf(d);
+    if (d2 > s || (d2 == s && ((int)r & 1))) r += copysignf(1.f, d);
+    return __float_as_uint(r + kMagic);
+}
+
+// 4 n values to n words of signed bytes (the low bytes of quantised floats' bits), rounding those next to a border exactly
+template <int N>
+__device__ __forceinline__ void quantise_pack(const float (&v)[N], float s, float inv, unsigned (&out)[N / 4]) {
+    constexpr float kMagic = 12582912.f;
+    unsigned m[N];
+    float near = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float t = v[i] * inv, k = t + kMagic;
+        near = fmaxf(near, fabsf(t - (k - kMagic)));
+        m[i] = __float_as_uint(k);
+    }
+    if (near > 0.4999f) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) m[i] = quantise_exact(v[i], s, inv);
+    }
+#pragma unroll
+    for (int j = 0; j < N / 4; ++j) {
+        const unsigned lo = __builtin_amdgcn_perm(m[4 * j + 1], m[4 * j], 0x0c0c0400u);
+        const unsigned hi = __builtin_amdgcn_perm(m[4 * j + 3], m[4 * j + 2], 0x0c0c0400u);
+        out[j] = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+    }
+}
+
+// A row's scale from its largest magnitude, given by its bits (a NaN is above an infinity, and that above every number): `given`
+// is what the caller gets, s and inv what the values are quantised with; !some: the row's bytes are zeros (a row below
+// 127 * 2^-126 counts as zero, so that s is a normal number; one with a NaN or an infinity has no scale).
+struct RowScale {
+    float given, s, inv;
+    bool some;
+};
+__device__ __forceinline__ RowScale row_scale(unsigned top) {
+    const float amax = __uint_as_float(top);
+    const bool bad = top >= 0x7f800000u;
+    RowScale r;
+    r.some = !bad && amax >= 127.f * 1.17549435e-38f;
+    r.s = !r.some ? 1.f : amax < 1e-25f ? amax / 127.f : quotient(amax, 127.f, 1.f / 127.f);
+    r.inv = __builtin_amdgcn_rcpf(r.s);
+    r.given = r.some ? r.s : bad ? __uint_as_float(0x7fc00000u) : 0.f;
+    return r;
+}
+
 // A piece: VEC consecutive values, 16 bytes.  Rows may begin at any value's address (gfx950 moves 16 bytes from and to any
 // address), so a row is dealt to the lanes the same way wherever it lies, and its result does not depend on that.  RAG: C is no
 // multiple of VEC, and the row's last piece, `n` < VEC values of it, is moved value by value (zeros behind it).

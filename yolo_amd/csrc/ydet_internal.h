@@ -111,6 +111,7 @@ int ydet_launch_focus_pair(const ydet_conv_desc* focus, const ydet_conv_desc* ne
 int ydet_launch_rgb_conv(const ydet_conv_desc* d, int x_dtype, hipStream_t stream);
 int ydet_launch_bottleneck(const ydet_conv_desc* c1, const ydet_conv_desc* c2, const ydet_conv_desc* c3 /* or null */, hipStream_t stream);
 int ydet_launch_layer_norm(const ydet_layer_norm_desc* d, hipStream_t stream);
+int ydet_check_quantize_rows(const ydet_quantize_desc* d);
 int ydet_launch_quantize_rows(const ydet_quantize_desc* d, hipStream_t stream);
 int ydet_launch_matmul_i8(const ydet_matmul_i8_desc* d, void* ws, size_t ws_bytes, hipStream_t stream);
 int ydet_launch_linear_i8(const ydet_quantize_desc* in, const ydet_matmul_i8_desc* product, void* ws, size_t ws_bytes, hipStream_t stream);

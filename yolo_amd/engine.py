@@ -728,8 +728,16 @@ class Plan:
                         op.conv.splitk_ws, op.conv.splitk_ws_bytes = ws.data_ptr(), ws.numel()
         # rows in 8 bits of the products (set_pointwise_int8): one workspace per launch list, likewise
         self.i8_ws = []
+
+        def i8_bytes(op):
+            saved, probe = (op.rows.x, op.product.y, op.product.res), 256      # (stand-ins for caller-owned maps, as above)
+            op.rows.x, op.product.y, op.product.res = (v or probe for v in saved)
+            n = int(_ffi.lib().ydet_linear_i8_workspace_bytes(C.byref(op.rows), C.byref(op.product)))
+            op.rows.x, op.product.y, op.product.res = saved
+            return n
+
         for ops in self.op_lists:
-            need = [_ffi.lib().ydet_linear_i8_workspace_bytes(op.rows.rows, op.rows.C) if op.kind == _ffi.OP_LINEAR_I8 else 0 for op in ops]
+            need = [i8_bytes(op) if op.kind == _ffi.OP_LINEAR_I8 else 0 for op in ops]
             ws = torch.empty(max(need), dtype=torch.uint8, device=g.device) if max(need, default=0) > 0 else None
             self.i8_ws.append(ws)
             for op, nb in zip(ops, need):

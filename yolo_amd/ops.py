@@ -289,18 +289,20 @@ MAX_ROW = 8192      # channels of a row that layer_norm and quantize_rows take
 
 def _launch(dev, call, *args):
     """`call(*args, stream)` on torch's current stream of `dev`."""
-    if torch.cuda.current_device() == dev.index:
-        return call(*args, torch._C._cuda_getCurrentRawStream(dev.index))
-    with torch.cuda.device(dev):
-        return call(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    i = dev.index
+    if torch.cuda.current_device() == i:
+        return call(*args, torch._C._cuda_getCurrentRawStream(i))
+    with torch.cuda.device(i):
+        return call(*args, torch._C._cuda_getCurrentRawStream(i))
 
 
 def _as_rows(t, what):
     """(t or a copy, rows, distance of rows) of a [..., C] tensor."""
-    if t.dim() == 0 or t.shape[-1] == 0:
-        raise ValueError(f"{what} needs at least one channel (shape {tuple(t.shape)})")
-    C = t.shape[-1]
-    n = t.numel() // C
+    shape = t.shape
+    if not shape or not shape[-1]:
+        raise ValueError(f"{what} needs at least one channel (shape {tuple(shape)})")
+    C = shape[-1]
+    n = shape[0] if len(shape) == 2 else t.numel() // C
     if t.is_contiguous():
         return t, n, C
     if t.stride(-1) == 1 or C == 1:
@@ -308,29 +310,29 @@ def _as_rows(t, what):
             ld = t.view(-1, C).stride(0) if n > 1 else C
         except RuntimeError:
             ld = 0
-        if C <= ld < 2 ** 31 and (C > 1 or n == 1 or ld >= 1):
+        if C <= ld < 2 ** 31:
             return t, n, ld
     return t.contiguous(), n, C
 
 
 def _params(C, dev, w, b):
     """The per-channel parameters (None allowed) as contiguous tensors of one type, and that type."""
-    dt = None
+    td = None
     for p in (w, b):
         if p is not None:
-            if p.dim() != 1 or p.shape[0] != C:
+            if p.shape != (C,):
                 raise ValueError(f"weight and bias have one value a channel: got {tuple(p.shape)} for {C} channels")
             if p.device != dev:
                 raise RuntimeError(f"weight / bias on {p.device}, the input on {dev}")
-            d = _dt(p)
-            dt = d if dt is None or dt == d else _ffi.F32
-    dt = _ffi.F32 if dt is None else dt
-    td = torch.float32 if dt == _ffi.F32 else torch.bfloat16
-    if w is not None and (w.dtype != td or not w.is_contiguous()):
+            d = p.dtype
+            if d is not torch.float32 and d is not torch.bfloat16:
+                raise TypeError(f"unsupported dtype {d}")
+            td = d if td is None or td is d else torch.float32
+    if w is not None and (w.dtype is not td or not w.is_contiguous()):
         w = w.detach().to(td).contiguous()
-    if b is not None and (b.dtype != td or not b.is_contiguous()):
+    if b is not None and (b.dtype is not td or not b.is_contiguous()):
         b = b.detach().to(td).contiguous()
-    return w, b, dt
+    return w, b, _ffi.BF16 if td is torch.bfloat16 else _ffi.F32
 
 
 def _ptr(t):
@@ -345,9 +347,13 @@ def _ln_forward(x, weight, bias, eps, stats):
     C, dev = x.shape[-1], x.device
     w, b, pdt = _params(C, dev, weight, bias)
     y = torch.empty(x.shape, device=dev, dtype=x.dtype)
-    st = torch.empty((2,) + x.shape[:-1], device=dev, dtype=torch.float32) if stats else None
-    mean = st.data_ptr() if stats else None
-    d = _ffi.LayerNormDesc(x.data_ptr(), y.data_ptr(), _ptr(w), _ptr(b), mean, mean and mean + 4 * n, n, C, ld, 0, C, 0, dt, pdt, eps)
+    st = mean = rstd = None
+    if stats:
+        st = torch.empty((2,) + x.shape[:-1], device=dev, dtype=torch.float32)
+        mean = st.data_ptr()
+        rstd = mean + 4 * n
+    d = _ffi.LayerNormDesc(x.data_ptr(), y.data_ptr(), w if w is None else w.data_ptr(), b if b is None else b.data_ptr(), mean, rstd,
+                           n, C, ld, 0, C, 0, dt, pdt, eps)
     rc = _launch(dev, _ffi.lib().ydet_layer_norm, d)
     if rc:
         _ffi.check(rc, "ydet_layer_norm")
@@ -427,7 +433,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Layer normalisation over the last dimension, differentiable in x, weight and bias (once).  A recorded graph cannot be
     captured (its leaves' gradients may belong to another stream): a captured training step calls layer_norm_forward and
     layer_norm_backward."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
         _need_cuda(x)
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("layer_norm: gradients are not recorded during graph capture; call layer_norm_forward and "
@@ -580,10 +587,10 @@ def linear_i8(x, lin, act="none", slope=0.1, res=None, res_mode="after", out_dty
     dt = _dt(x)
     x, n, ld = _as_rows(x, "linear_i8")
     y, d, keep = _product(None, None, n, 0, lin, act, slope, res, res_mode, x.dtype if out_dtype is None else out_dtype)
-    nbytes = lib.ydet_linear_i8_workspace_bytes(n, K)
-    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
     src = _ffi.QuantizeDesc(x.data_ptr(), None, None, None, None, n, K, ld, 0, 0, dt, _ffi.F32, 0, 0.0)
-    rc = _launch(dev, lib.ydet_linear_i8, src, d, ws.data_ptr(), nbytes)
+    nbytes = lib.ydet_linear_i8_workspace_bytes(src, d)
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+    rc = _launch(dev, lib.ydet_linear_i8, src, d, _ptr(ws), nbytes)
     if rc:
         _ffi.check(rc, "ydet_linear_i8")
     return y if len(lead) == 1 else y.view(lead + (lin.N,))
