@@ -697,3 +697,115 @@ def test_plan_in_8_bits_replicas_and_graph(pointwise_int8):
         want = one.run(xk)["y"].clone()
         assert torch.equal(replay(xk), want)
         torch.cuda.synchronize()
+
+
+# ---- calls at the edges -------------------------------------------------------------------------------------------------------
+def test_second_derivative_is_an_error():
+    x = torch.randn(4, 24, device=DEV, requires_grad=True)
+    w = torch.randn(24, device=DEV, requires_grad=True)
+    gx, = torch.autograd.grad(ops.layer_norm(x, w).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        gx.sum().backward()
+    gx, = torch.autograd.grad(ops.layer_norm(x, w).square().sum(), x)
+    assert not gx.requires_grad
+
+
+def test_input_changed_behind_the_forward_pass_is_an_error():
+    x = torch.randn(4, 24, device=DEV)
+    w = torch.randn(24, device=DEV, requires_grad=True)
+    y = ops.layer_norm(x, w)
+    x.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_products_without_rows_and_single_rows():
+    lin = ops.LinearI8.quantize(torch.randn(20, 30, device=DEV))
+    for lead in ((0,), (3, 0), (0, 5)):
+        q, s = ops.quantize_rows(torch.empty(*lead, 30, device=DEV))
+        assert ops.matmul_i8(q, s, lin).shape == lead + (20,)
+        assert ops.linear_i8(torch.empty(*lead, 30, device=DEV), lin, res=torch.empty(*lead, 20, device=DEV)).shape == lead + (20,)
+    x = torch.randn(30, device=DEV)
+    q, s = ops.quantize_rows(x)
+    assert q.shape == (30,) and s.shape == ()
+    y = ops.matmul_i8(q, s, lin, out_dtype=F32)
+    assert y.shape == (20,) and torch.equal(y, ops.linear_i8(x, lin)) and torch.equal(y, ops.linear_i8(x[None, None], lin)[0, 0])
+    y, m, r = ops.layer_norm_forward(x)
+    assert y.shape == (30,) and m.shape == r.shape == ()
+    assert torch.equal(ops.layer_norm_backward(y, x, m, r)[0], ops.layer_norm_backward(y[None], x[None], m[None], r[None])[0][0])
+
+
+@pytest.mark.parametrize("M", [65, 127, 129, 191, 193, 255, 257, 321])
+def test_tails_of_every_tile(M):
+    """The last rows of a tile, the scales behind them and the last channels, for K on both sides of the kernels' choices."""
+    g = gen(M)
+    for reps, K, N in ((1, 2048, 8), (40, 1024, 320), (130, 2050, 1100), (100, 130, 520), (300, 64, 72)):
+        rows = M * reps + M % 7
+        q, s, wq, ws, bias = operands(g, rows, K, N)
+        lin = ops.LinearI8(wq, ws, bias)
+        y = ops.matmul_i8(q, s, lin, act="leaky", out_dtype=F32)
+        # (the last rows and a few others: the whole product in 64 bits would take long)
+        some = torch.cat([torch.arange(0, rows, max(1, rows // 50), device=DEV), torch.arange(max(0, rows - 200), rows, device=DEV)])
+        want, e = product64(q[some], s[some], wq, ws, bias, "leaky", 0.1, None, "after")
+        within(y[some], want, e + half(F32) * (want.abs() + e) + 1e-37)
+
+
+def test_outputs_leave_the_rest_alone():
+    """Output slices of wider maps, through the library: the channels beside and the rows behind them stay as they were."""
+    g = gen(9)
+    lib, st = _ffi.lib(), _ffi.current_stream()
+    for rows, K, N, coff in ((5, 77, 30, 3), (700, 128, 72, 8), (40000, 64, 64, 1), (7000, 1024, 200, 5)):
+        ld = N + coff + 7
+        q, s, wq, ws, bias = operands(g, rows, K, N)
+        lin = ops.LinearI8(wq, ws, bias)
+        q, s = ops.quantize_rows(q.float() * s[:, None])
+        want = ops.matmul_i8(q, s, lin, out_dtype=F32)
+        buf = torch.full((rows + 9, ld), -7.0, device=DEV)
+        d = _ffi.MatmulI8Desc(q.data_ptr(), s.data_ptr(), lin.w.data_ptr(), lin.scale.data_ptr(), lin.bias.data_ptr(), None, buf.data_ptr(), rows, K,
+                              N, lin.kp, lin.n_pad, q.stride(0), 0, ld, coff, 0, 0, 0, 0.0, 0, _ffi.F32)
+        _ffi.check(lib.ydet_matmul_i8(d, None, 0, st))
+        assert torch.equal(buf[:rows, coff:coff + N], want)
+        buf[:rows, coff:coff + N] = -7.0
+        assert (buf == -7.0).all()
+    for C, dtype in ((30, F32), (30, BF16), (512, BF16), (2049, F32)):
+        x = randn(g, 50, C, dtype=dtype)
+        want = ops.layer_norm(x)
+        buf = torch.full((53, C + 9), -7.0, device=DEV, dtype=dtype)
+        d = _ffi.LayerNormDesc(x.data_ptr(), buf.data_ptr(), None, None, None, None, 50, C, C, 0, C + 9, 4, ops._dt(x), 0, 1e-5)
+        _ffi.check(lib.ydet_layer_norm(d, st))
+        assert torch.equal(buf[:50, 4:C + 4], want)
+        buf[:50, 4:C + 4] = -7.0
+        assert (buf == -7.0).all()
+        Cp = (C + 15) // 16 * 16
+        qb = torch.full((53, Cp + 16), -7, device=DEV, dtype=torch.int8)
+        sb = torch.full((53,), -7.0, device=DEV)
+        d = _ffi.QuantizeDesc(x.data_ptr(), qb.data_ptr(), sb.data_ptr(), None, None, 50, C, C, 0, Cp + 16, ops._dt(x), 0, 0, 0.0)
+        _ffi.check(lib.ydet_quantize_rows_i8(d, st))
+        q, s = ops.quantize_rows(x)
+        assert torch.equal(qb[:50, :C], q) and torch.equal(sb[:50], s) and not qb[:50, C:Cp].any()
+        assert (qb[:, Cp:] == -7).all() and (qb[50:] == -7).all() and (sb[50:] == -7).all()
+
+
+def test_in_place():
+    """y may be x, dx may be dy, and a product's output its residual."""
+    g = gen(10)
+    x, dy = randn(g, 900, 40, dtype=BF16), randn(g, 900, 40, dtype=BF16)
+    lib, st = _ffi.lib(), _ffi.current_stream()
+    y, m, r = ops.layer_norm_forward(x)
+    dx, _, _ = ops.layer_norm_backward(dy, x, m, r, need=(True, False, False))
+    d2 = dy.clone()
+    d = _ffi.LayerNormGradDesc(d2.data_ptr(), x.data_ptr(), d2.data_ptr(), None, m.data_ptr(), r.data_ptr(), None, None, 900, 40, 40, 0, 40, 0, 40, 0,
+                               _ffi.BF16, 0)
+    _ffi.check(lib.ydet_layer_norm_backward(d, None, 0, st))
+    assert torch.equal(d2, dx)
+    x2 = x.clone()
+    _ffi.check(lib.ydet_layer_norm(_ffi.LayerNormDesc(x2.data_ptr(), x2.data_ptr(), None, None, None, None, 900, 40, 40, 0, 40, 0, _ffi.BF16, 0, 1e-5), st))
+    assert torch.equal(x2, y)
+    lin = ops.LinearI8.quantize(randn(g, 40, 40))
+    q, s = ops.quantize_rows(x)
+    want = ops.matmul_i8(q, s, lin, act="silu", res=x)
+    x3 = x.clone()
+    d = _ffi.MatmulI8Desc(q.data_ptr(), s.data_ptr(), lin.w.data_ptr(), lin.scale.data_ptr(), None, x3.data_ptr(), x3.data_ptr(), 900, 40, 40, lin.kp,
+                          lin.n_pad, q.stride(0), 0, 40, 0, 40, 0, _ffi.ACT_SILU, 0.0, _ffi.RES_AFTER_ACT, _ffi.BF16)
+    _ffi.check(lib.ydet_matmul_i8(d, None, 0, st))
+    assert torch.equal(x3, want)

@@ -186,11 +186,13 @@ __global__ __launch_bounds__(64 * WAVES_N * WAVES_M, 2) void tile_kernel(const A
                                                                             0x00020000);
         for (int k = wave; k < (2 * BN + BM) / 64; k += NW) {
             __attribute__((address_space(3))) void* dst = (__attribute__((address_space(3))) void*)(sc + k * 64);
-            if (k < BN / 64) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, dst, 4, lane * 4, k * 256, 0, 0);
-            else if (k < 2 * BN / 64) __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, dst, 4, lane * 4, (k - BN / 64) * 256, 0, 0);
-            else __builtin_amdgcn_raw_ptr_buffer_load_lds(rr, dst, 4, lane * 4, (k - 2 * BN / 64) * 256, 0, 0);
+            // (whole offsets in the vector register: they may lie behind the extent, where zeros are read)
+            if (k < BN / 64) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, dst, 4, (k * 64 + lane) * 4, 0, 0, 0);
+            else if (k < 2 * BN / 64) __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, dst, 4, ((k - BN / 64) * 64 + lane) * 4, 0, 0, 0);
+            else __builtin_amdgcn_raw_ptr_buffer_load_lds(rr, dst, 4, ((k - 2 * BN / 64) * 64 + lane) * 4, 0, 0, 0);
         }
     }
+    // (kt's part may ride in the scalar offset: it lies below every extent, of at least one row's K and of one channel's kp)
     auto issue = [&](int stage, int kt) {
         kt *= RB;
         char* dst = stages + stage * STAGE + wave * 1024;
@@ -543,7 +545,8 @@ __global__ __launch_bounds__(256) void align_rows_kernel(const char* x, long lon
 //     1600 x 512 -> 512: 6.7 against 4.5);
 //   256 x 192 tiles for K >= 2048 where they leave no quarter of the CUs idle (23104 x 4096 -> 512: 52, in 128 x 128 tiles 73; but
 //     25600 x 1024 -> 512: 32 against 25);
-//   128 x 128 for K >= 1024 with at least a tile a CU (6400 x 1024 -> 1024: 14.1, in 64 x 128 tiles 16.4);
+//   128 x 128 for K >= 1024 with at least a tile a CU (6400 x 1024 -> 1024: 13.3, in 64 x 128 tiles 16.4; with four waves instead of
+//     eight 13.6);
 //   64 x 128 otherwise (409600 x 64 -> 64: 18, in 128 x 128 tiles 28; 409600 x 128 -> 128 with residual: 52 against 62), with a
 //     third stage where there are fewer than two workgroups a CU (2888 x 4096 -> 512: 14.6, with two stages 19.2).
 // The tile kernels want rows in 16-byte pieces: others are first copied into the workspace.
@@ -568,7 +571,7 @@ static int launch(const Args& a, bool wide_x, hipStream_t stream) {
     if (direct == 16) return wide_x ? launch_few<OUT, 1, 1, 8, false>(a, stream) : launch_few<OUT, 1, 1, 8, true>(a, stream);
     if (direct == 32) return wide_x ? launch_few<OUT, 2, 2, 4, false>(a, stream) : launch_few<OUT, 2, 2, 4, true>(a, stream);
     if (a.K >= 2048 && a.N > 128 && tiles(a, 256, 192) * 4 >= cus * 3) return launch_tile<OUT, 256, 192, 2, 4>(a, stream);
-    if (a.K >= 1024 && a.N > 64 && tiles(a, 128, 128) >= cus) return launch_tile<OUT, 128, 128, 2, 2>(a, stream);
+    if (a.K >= 1024 && a.N > 64 && tiles(a, 128, 128) >= cus) return launch_tile<OUT, 128, 128, 2, 4>(a, stream);
     if (tiles(a, 64, 128) < 2 * cus) return launch_tile<OUT, 64, 128, 1, 4, 3>(a, stream);
     return launch_tile<OUT, 64, 128, 1, 4, 2>(a, stream);
 }

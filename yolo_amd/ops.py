@@ -539,7 +539,7 @@ def _product(x, scale, n, ld, lin, act, slope, res, res_mode, out_dtype):
 def matmul_i8(q, scale, lin, act="none", slope=0.1, res=None, res_mode="after", out_dtype=torch.bfloat16):
     """act(q . lin.w^T * scale * lin.scale + lin.bias), [..., N] of out_dtype (bf16 or fp32), from int8 rows q [..., K] and
     their scales [...] (quantize_rows).  act: "none", "leaky" (negative slope `slope`), "silu".  res [..., N] of out_dtype is
-    added after or before the activation (res_mode).  The sums are exact integers."""
+    added after or before the activation (res_mode).  The sums are exact integers.  (For inference: no gradients.)"""
     _need_cuda(q, scale)
     K, shape = lin.K, q.shape
     if q.dtype != torch.int8 or len(shape) == 0 or shape[-1] != K:
@@ -572,7 +572,8 @@ def matmul_i8(q, scale, lin, act="none", slope=0.1, res=None, res_mode="after", 
 
 
 def linear_i8(x, lin, act="none", slope=0.1, res=None, res_mode="after", out_dtype=None):
-    """matmul_i8 of a floating map x [..., K], whose rows are quantised (quantize_rows) on the way; out_dtype defaults to x's."""
+    """matmul_i8 of a floating map x [..., K], whose rows are quantised (quantize_rows) on the way; out_dtype defaults to x's.
+    The same bits as the two calls; K up to MAX_ROW."""
     _need_cuda(x)
     K, shape = lin.K, x.shape
     if shape[-1:] != (K,):
