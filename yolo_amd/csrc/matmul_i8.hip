@@ -484,9 +484,15 @@ __global__ __launch_bounds__(512) void few_float_rows_kernel(const Args a) {
         if (wave + u * NW >= steps) break;
         float v[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = rs.some ? (float)raw[u][i / VEC][i % VEC] : 0.f;
-        unsigned d[4];
-        quantise_pack(v, rs.s, rs.inv, d);
+        for (int i = 0; i < 16; ++i) v[i] = (float)raw[u][i / VEC][i % VEC];
+        unsigned m[16], d[4];
+        if (quantise_near(v, rs.inv, m) > 0.4999f) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) m[i] = quantise_exact(v[i], rs.s, rs.inv);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m[i] = rs.bad ? 0u : m[i];
+        pack_bytes(m, d);
         acc[0][0] = mma(fa[u], i32x4{(int)d[0], (int)d[1], (int)d[2], (int)d[3]}, acc[0][0]);
     }
     const float xs[1] = {rs.given};

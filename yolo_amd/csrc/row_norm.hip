@@ -63,76 +63,115 @@ __global__ __launch_bounds__(kThreads) void row_norm_kernel(const RowArgs a) {
                 if (row < a.rows && col < a.C) in[r][c] = P::load(xr + col, a.C - col);
             }
         }
+        // (step by step over all RPT rows, whose chains of operations fill each other's gaps)
+        float v[RPT][CH * VEC];
 #pragma unroll
-        for (int r = 0; r < RPT; ++r) {
-            const long long row = row0 + r * G + g;
-            const bool live = row < a.rows;
-            float v[CH * VEC];
+        for (int r = 0; r < RPT; ++r)
 #pragma unroll
             for (int c = 0; c < CH; ++c)
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) v[c * VEC + i] = (float)in[r][c][i];
-            if constexpr (NORM) {
-                float sum = 0.f;
+                for (int i = 0; i < VEC; ++i) v[r][c * VEC + i] = (float)in[r][c][i];
+        if constexpr (NORM) {
+            float mean[RPT], rstd[RPT];
 #pragma unroll
-                for (int i = 0; i < CH * VEC; ++i) sum += v[i];
-                const float mean = quotient(group_sum<LPR>(sum, red, slot), fc, a.inv_c);
-                float sq = 0.f;
+            for (int r = 0; r < RPT; ++r) {
+                mean[r] = 0.f;
+#pragma unroll
+                for (int i = 0; i < CH * VEC; ++i) mean[r] += v[r][i];
+            }
+#pragma unroll
+            for (int r = 0; r < RPT; ++r) mean[r] = quotient(group_sum<LPR>(mean[r], red, slot), fc, a.inv_c);
+#pragma unroll
+            for (int r = 0; r < RPT; ++r) {
+                rstd[r] = 0.f;
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
                     const int left = a.C - (c * LPR + l) * VEC;
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) {
-                        const float d = P::has(i, left) ? v[c * VEC + i] - mean : 0.f;
-                        v[c * VEC + i] = d;
-                        sq = fmaf(d, d, sq);
+                        const float d = P::has(i, left) ? v[r][c * VEC + i] - mean[r] : 0.f;
+                        v[r][c * VEC + i] = d;
+                        rstd[r] = fmaf(d, d, rstd[r]);
                     }
                 }
-                const float rstd = __builtin_amdgcn_rsqf(fmaf(group_sum<LPR>(sq, red, slot), a.inv_c, a.eps));
-                if (a.mean && live && l == 0) {
-                    a.mean[row] = mean;
-                    a.rstd[row] = rstd;
-                }
-#pragma unroll
-                for (int i = 0; i < CH * VEC; ++i) v[i] = P::has(i % VEC, a.C - (i / VEC * LPR + l) * VEC) ? fmaf(v[i] * rstd, w[i], b[i]) : 0.f;
             }
-            if constexpr (!QUANT) {
-                if (live) {
-                    T* yr = reinterpret_cast<T*>(a.y) + row * a.y_ld;
 #pragma unroll
-                    for (int c = 0; c < CH; ++c) {
-                        const int col = (c * LPR + l) * VEC;
-                        if (col < a.C) {
-                            typename P::type o;
+            for (int r = 0; r < RPT; ++r) rstd[r] = __builtin_amdgcn_rsqf(fmaf(group_sum<LPR>(rstd[r], red, slot), a.inv_c, a.eps));
+            if (a.mean && l == 0) {
 #pragma unroll
-                            for (int i = 0; i < VEC; ++i) o[i] = (T)v[c * VEC + i];
-                            P::store(yr + col, o, a.C - col);
-                        }
+                for (int r = 0; r < RPT; ++r) {
+                    const long long row = row0 + r * G + g;
+                    if (row < a.rows) a.mean[row] = mean[r], a.rstd[row] = rstd[r];
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < RPT; ++r)
+#pragma unroll
+                for (int i = 0; i < CH * VEC; ++i)
+                    v[r][i] = P::has(i % VEC, a.C - (i / VEC * LPR + l) * VEC) ? fmaf(v[r][i] * rstd[r], w[i], b[i]) : 0.f;
+        }
+        if constexpr (!QUANT) {
+#pragma unroll
+            for (int r = 0; r < RPT; ++r) {
+                const long long row = row0 + r * G + g;
+                if (row >= a.rows) continue;
+                T* yr = reinterpret_cast<T*>(a.y) + row * a.y_ld;
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    const int col = (c * LPR + l) * VEC;
+                    if (col < a.C) {
+                        typename P::type o;
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) o[i] = (T)v[r][c * VEC + i];
+                        P::store(yr + col, o, a.C - col);
                     }
                 }
-            } else {
-                // (lanes and pieces behind the row's end hold zeros)
-                unsigned top = 0;
+            }
+        } else {
+            // (lanes and pieces behind the row's end hold zeros)
+            unsigned top[RPT], m[RPT][CH * VEC];
+            RowScale rs[RPT];
+            float near = 0.f;
+            bool bad = false;
 #pragma unroll
-                for (int i = 0; i < CH * VEC; ++i) {
-                    const unsigned u = __float_as_uint(v[i]) & 0x7fffffffu;
-                    top = u > top ? u : top;
-                }
-                const RowScale rs = row_scale(group_reduce<LPR>(top, MaxU{}, red, slot));
-                if (live && l == 0) a.scale[row] = rs.given;
+            for (int r = 0; r < RPT; ++r) {
+                top[r] = 0;
 #pragma unroll
-                for (int i = 0; i < CH * VEC; ++i) v[i] = rs.some ? v[i] : 0.f;
+                for (int i = 0; i < CH * VEC; ++i) top[r] = MaxU{}(top[r], __float_as_uint(v[r][i]) & 0x7fffffffu);
+            }
+#pragma unroll
+            for (int r = 0; r < RPT; ++r) rs[r] = row_scale(group_reduce<LPR>(top[r], MaxU{}, red, slot));
+#pragma unroll
+            for (int r = 0; r < RPT; ++r) {
+                near = fmaxf(near, quantise_near(v[r], rs[r].inv, m[r]));
+                bad = bad || rs[r].bad;
+            }
+            if (near > 0.4999f) {
+#pragma unroll
+                for (int r = 0; r < RPT; ++r)
+#pragma unroll
+                    for (int i = 0; i < CH * VEC; ++i) m[r][i] = quantise_exact(v[r][i], rs[r].s, rs[r].inv);
+            }
+            if (bad) {
+#pragma unroll
+                for (int r = 0; r < RPT; ++r)
+#pragma unroll
+                    for (int i = 0; i < CH * VEC; ++i) m[r][i] = rs[r].bad ? 0u : m[r][i];
+            }
+#pragma unroll
+            for (int r = 0; r < RPT; ++r) {
+                const long long row = row0 + r * G + g;
+                if (row >= a.rows) continue;
+                if (l == 0) a.scale[row] = rs[r].given;
                 unsigned d[CH * VEC / 4];
-                quantise_pack(v, rs.s, rs.inv, d);
-                if (live) {
-                    char* yr = a.y + row * a.y_ld;
+                pack_bytes(m[r], d);
+                char* yr = a.y + row * a.y_ld;
 #pragma unroll
-                    for (int c = 0; c < CH; ++c) {
-                        const int col = (c * LPR + l) * VEC;
-                        if (col < a.cw) {
-                            if constexpr (VEC == 8) *reinterpret_cast<uint2*>(yr + col) = make_uint2(d[2 * c], d[2 * c + 1]);
-                            else *reinterpret_cast<unsigned*>(yr + col) = d[c];
-                        }
+                for (int c = 0; c < CH; ++c) {
+                    const int col = (c * LPR + l) * VEC;
+                    if (col < a.cw) {
+                        if constexpr (VEC == 8) *reinterpret_cast<uint2*>(yr + col) = make_uint2(d[2 * c], d[2 * c + 1]);
+                        else *reinterpret_cast<unsigned*>(yr + col) = d[c];
                     }
                 }
             }
@@ -153,10 +192,11 @@ static int launch_rows(const RowArgs& a, hipStream_t stream) {
     return YDET_OK;
 }
 
-// Rows a lane group takes at once: four (their loads in flight together) where that still leaves eight workgroups a CU, else one.
+// Rows a lane group takes at once: four (their loads in flight together) where that still leaves eight workgroups a CU, else one;
+// one where the rows are quantised (four cost 148 registers: 102400 x 256 norm + quantisation 28.2 us, with one 20.4).
 template <int MODE, typename T, bool RAG, int LPR, int CH>
 static int launch_depth(const RowArgs& a, hipStream_t stream) {
-    if constexpr (CH == 1) {
+    if constexpr (CH == 1 && !(MODE & kQuant)) {
         if (a.rows >= (long long)current_device_info().cus * 8 * 4 * (kThreads / LPR))
             return launch_rows<MODE, T, RAG, LPR, CH, 4>(a, stream);
     }

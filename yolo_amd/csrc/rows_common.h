@@ -33,7 +33,7 @@ static inline Shape shape_of(int cols, int vec) {
 
 template <int CTRL>
 __device__ __forceinline__ unsigned dpp(unsigned v) {
-    return (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
+    return (unsigned)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);      // (every lane has a source)
 }
 // Combines the LPR <= 64 lanes of a group so that every lane holds the result; op is commutative and the tree is the same for
 // every lane, so all lanes hold the same bits.  Neighbours by DPP inside 16 lanes, then by the lane-row swaps.
@@ -101,22 +101,21 @@ __device__ __forceinline__ unsigned quantise_exact(float v, float s, float inv) 
     return __float_as_uint(r + kMagic);
 }
 
-// 4 n values to n words of signed bytes (the low bytes of quantised floats' bits), rounding those next to a border exactly
+// N values to N / 4 words of signed bytes; values next to a border (a lane's, seldom) are rounded exactly.
+constexpr float kRound = 12582912.f;        // 1.5 * 2^23: a float of this size has its integer in the low bits
 template <int N>
-__device__ __forceinline__ void quantise_pack(const float (&v)[N], float s, float inv, unsigned (&out)[N / 4]) {
-    constexpr float kMagic = 12582912.f;
-    unsigned m[N];
+__device__ __forceinline__ float quantise_near(const float (&v)[N], float inv, unsigned (&m)[N]) {
     float near = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const float t = v[i] * inv, k = t + kMagic;
-        near = fmaxf(near, fabsf(t - (k - kMagic)));
+        const float t = v[i] * inv, k = t + kRound;
+        near = fmaxf(near, fabsf(t - (k - kRound)));
         m[i] = __float_as_uint(k);
     }
-    if (near > 0.4999f) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) m[i] = quantise_exact(v[i], s, inv);
-    }
+    return near;
+}
+template <int N>
+__device__ __forceinline__ void pack_bytes(const unsigned (&m)[N], unsigned (&out)[N / 4]) {
 #pragma unroll
     for (int j = 0; j < N / 4; ++j) {
         const unsigned lo = __builtin_amdgcn_perm(m[4 * j + 1], m[4 * j], 0x0c0c0400u);
@@ -126,20 +125,20 @@ __device__ __forceinline__ void quantise_pack(const float (&v)[N], float s, floa
 }
 
 // A row's scale from its largest magnitude, given by its bits (a NaN is above an infinity, and that above every number): `given`
-// is what the caller gets, s and inv what the values are quantised with; !some: the row's bytes are zeros (a row below
-// 127 * 2^-126 counts as zero, so that s is a normal number; one with a NaN or an infinity has no scale).
+// is what the caller gets, s and inv what the values are quantised with.  A row below 127 * 2^-126 counts as zero, so that s is
+// a normal number: its inv is 0, and so are its values.  bad: the row has a NaN or an infinity, hence no scale, and zeros.
 struct RowScale {
     float given, s, inv;
-    bool some;
+    bool bad;
 };
 __device__ __forceinline__ RowScale row_scale(unsigned top) {
     const float amax = __uint_as_float(top);
-    const bool bad = top >= 0x7f800000u;
     RowScale r;
-    r.some = !bad && amax >= 127.f * 1.17549435e-38f;
-    r.s = !r.some ? 1.f : amax < 1e-25f ? amax / 127.f : quotient(amax, 127.f, 1.f / 127.f);
-    r.inv = __builtin_amdgcn_rcpf(r.s);
-    r.given = r.some ? r.s : bad ? __uint_as_float(0x7fc00000u) : 0.f;
+    r.bad = top >= 0x7f800000u;
+    const bool some = !r.bad && amax >= 127.f * 1.17549435e-38f;
+    r.s = !some ? 1.f : amax < 1e-25f ? amax / 127.f : quotient(amax, 127.f, 1.f / 127.f);
+    r.inv = some ? __builtin_amdgcn_rcpf(r.s) : 0.f;
+    r.given = some ? r.s : r.bad ? __uint_as_float(0x7fc00000u) : 0.f;
     return r;
 }
 
