@@ -548,10 +548,10 @@ typedef struct {
 size_t ydet_matmul_i8_workspace_bytes(const ydet_matmul_i8_desc* d);
 int ydet_matmul_i8(const ydet_matmul_i8_desc* d, void* workspace, size_t workspace_bytes, void* stream);
 
-/* ydet_quantize_rows_i8 and ydet_matmul_i8 behind each other, with the same result: `in` without q, scale and q_ld, `product`
- * without x, x_scale, x_ld and x_coff; in->rows == product->rows, in->C == product->K.  Few rows take one launch; otherwise the
- * 8-bit rows go to the caller's workspace (ydet_linear_i8_workspace_bytes, 16-byte aligned; 0: none, also for a pair that
- * ydet_linear_i8 refuses). */
+/* ydet_quantize_rows_i8 (normalize included) and ydet_matmul_i8 behind each other, with the same result: `in` without q, scale
+ * and q_ld, `product` without x, x_scale, x_ld and x_coff; in->rows == product->rows, in->C == product->K.  Few rows take one
+ * launch; otherwise the 8-bit rows go to the caller's workspace (ydet_linear_i8_workspace_bytes, 16-byte aligned; 0: none,
+ * also for a pair that ydet_linear_i8 refuses). */
 size_t ydet_linear_i8_workspace_bytes(const ydet_quantize_desc* in, const ydet_matmul_i8_desc* product);
 int ydet_linear_i8(const ydet_quantize_desc* in, const ydet_matmul_i8_desc* product, void* workspace, size_t workspace_bytes,
                    void* stream);

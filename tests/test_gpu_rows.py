@@ -700,6 +700,23 @@ def test_plan_in_8_bits_replicas_and_graph(pointwise_int8):
 
 
 # ---- calls at the edges -------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("M,K,N,dtype", [(5, 64, 32, BF16), (3000, 200, 130, F32)])
+def test_norm_and_product_in_one_call_of_the_library(M, K, N, dtype):
+    g = gen(K)
+    x, w, b = randn(g, M, K, dtype=dtype), 1 + 0.3 * randn(g, K), randn(g, K)
+    lin = ops.LinearI8.quantize(randn(g, N, K), randn(g, N))
+    want = ops.matmul_i8(*ops.layer_norm_quantize(x, w, b), lin, act="silu", out_dtype=F32)
+    y = torch.empty(M, N, device=DEV)
+    q = _ffi.QuantizeDesc(x.data_ptr(), None, None, w.data_ptr(), b.data_ptr(), M, K, K, 0, 0, ops._dt(x), _ffi.F32, 1, 1e-5)
+    d = _ffi.MatmulI8Desc(None, None, lin.w.data_ptr(), lin.scale.data_ptr(), lin.bias.data_ptr(), None, y.data_ptr(), M, K, N, lin.kp, lin.n_pad,
+                          0, 0, N, 0, 0, 0, _ffi.ACT_SILU, 0.0, 0, _ffi.F32)
+    lib = _ffi.lib()
+    n = lib.ydet_linear_i8_workspace_bytes(q, d)
+    ws = torch.empty(n, device=DEV, dtype=torch.uint8)
+    _ffi.check(lib.ydet_linear_i8(q, d, ws.data_ptr(), n, _ffi.current_stream()))
+    assert n > 0 and torch.equal(y, want)
+
+
 def test_second_derivative_is_an_error():
     x = torch.randn(4, 24, device=DEV, requires_grad=True)
     w = torch.randn(24, device=DEV, requires_grad=True)
