@@ -463,7 +463,8 @@ int ydet_preprocess_u8(const ydet_u8_image* images /* device, N entries */, cons
 /* Layer normalisation: y = (x - mean) * rstd * gamma + beta with the mean and variance of each row's C values,
  * rstd = 1 / sqrt(var + eps).  gamma / beta: C values of param_dtype, or NULL (1 / 0).  mean, rstd (rows values each, fp32,
  * both or neither): what the backward pass needs.  y has x's dtype; y may be x.  C <= 8192, rows < 2^31; any ld,
- * and slices at any value's address (a row's result does not depend on where it lies). */
+ * and slices at any value's address (a row's result does not depend on where it lies).  eps >= 0; with eps 0 a row whose
+ * variance is below 2^-126 counts as constant: its rstd is infinite. */
 typedef struct {
     const void* x;
     void* y;
@@ -524,6 +525,7 @@ int ydet_quantize_rows_i8(const ydet_quantize_desc* d, void* stream);
 /* Product in 8-bit integers -- a 1x1 convolution over rows that ydet_quantize_rows_i8 wrote:
  *   acc[r, n] = sum_k x[r, k] * w[n, k]      (exact 32-bit integers; K <= 131071)
  *   y[r, n]   = act(acc * x_scale[r] * w_scale[n] + bias[n])  with the residual as in ydet_conv2d_nhwc (res_mode; res has y's dtype)
+ * (in fp32 from the left: acc * x_scale[r] has to stay finite).
  * w [n_pad][kp], rows >= N and columns >= K zero, n_pad a multiple of 128, kp a multiple of 64; w_scale and bias (may be NULL)
  * hold n_pad values; all three 16-byte aligned.  Slices that are 16-byte aligned with x_ld a multiple of 16 are read in
  * 16-byte pieces (the bytes behind K in a row's last piece are read, their values do not matter; the slice's row has to hold

@@ -717,6 +717,25 @@ def test_norm_and_product_in_one_call_of_the_library(M, K, N, dtype):
     assert n > 0 and torch.equal(y, want)
 
 
+@pytest.mark.parametrize("wdt,bdt", [(BF16, F32), (F32, BF16)])
+def test_gradients_of_parameters_of_two_types(wdt, bdt):
+    # either gradient is rounded to its own parameter's type alone
+    rows, C = 300, 96
+    g = gen(7)
+    x, dy = randn(g, rows, C), randn(g, rows, C)
+    w, b = (1 + 0.3 * randn(g, C)).to(wdt).requires_grad_(), randn(g, C).to(bdt).requires_grad_()
+    ops.layer_norm(x, w, b).backward(dy)
+    xd, dyd = x.double(), dy.double()
+    xh = (xd - xd.mean(-1, keepdim=True)) / (xd.var(-1, keepdim=True, unbiased=False) + 1e-5).sqrt()
+    for got, terms, size, dt in ((w.grad, dyd * xh, dyd.abs() * (xh.abs() + 2 * xd.abs() + 1), wdt), (b.grad, dyd, dyd.abs(), bdt)):
+        assert got.dtype == dt
+        want = terms.sum(0)
+        # fp32 sums of `rows` terms, no chain of additions longer than their number; x-hat is off by a few steps of itself (the
+        # deviation) and of |x| and the mean (|mean| < 1/2, 1 / deviation < 2); then one rounding to the parameter's type
+        tol = (rows + 16) * 2.0 ** -24 * size.sum(0) + (2.0 ** -8 * want.abs() if dt is BF16 else 0)
+        assert ((got.double() - want).abs() <= tol).all()
+
+
 def test_second_derivative_is_an_error():
     x = torch.randn(4, 24, device=DEV, requires_grad=True)
     w = torch.randn(24, device=DEV, requires_grad=True)

@@ -93,16 +93,16 @@ __device__ __forceinline__ float quotient(float a, float b, float y) {
 // is within 3e-5 of the quotient, so rounding it (adding 1.5 * 2^23 leaves the integer in the low bits) is right unless it
 // lies that close to a border; there the remainder decides, which the fused multiply-add gives without error: near a
 // border |v - r s| is about s / 2 and a multiple of s's last place.
+constexpr float kRound = 12582912.f;        // 1.5 * 2^23
 __device__ __forceinline__ unsigned quantise_exact(float v, float s, float inv) {
-    constexpr float kMagic = 12582912.f;
-    float r = (v * inv + kMagic) - kMagic;
+    float r = (v * inv + kRound) - kRound;
     const float d = fmaf(-r, s, v), d2 = 2.f * fabsf(d);
     if (d2 > s || (d2 == s && ((int)r & 1))) r += copysignf(1.f, d);
-    return __float_as_uint(r + kMagic);
+    return __float_as_uint(r + kRound);
 }
 
-// N values to N / 4 words of signed bytes; values next to a border (a lane's, seldom) are rounded exactly.
-constexpr float kRound = 12582912.f;        // 1.5 * 2^23: a float of this size has its integer in the low bits
+// N values rounded the quick way into m; returns how far the worst of them lies from its integer, for the caller to round all
+// exactly where one is next to a border (seldom).  pack_bytes: the low bytes of N such values as N / 4 words.
 template <int N>
 __device__ __forceinline__ float quantise_near(const float (&v)[N], float inv, unsigned (&m)[N]) {
     float near = 0.f;

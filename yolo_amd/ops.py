@@ -362,7 +362,8 @@ def _ln_forward(x, weight, bias, eps, stats):
 
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
     """Layer normalisation over the last dimension: (y, mean, rstd), y of x's dtype and shape, mean and rstd fp32 of
-    x.shape[:-1].  weight, bias: [C] fp32 or bf16, or None."""
+    x.shape[:-1].  weight, bias: [C] fp32 or bf16, or None.  The variance is an fp32 number: with eps = 0 a row whose variance
+    is below 1.2e-38 counts as constant, and what is divided by its deviation is not finite."""
     y, st = _ln_forward(x, weight, bias, eps, True)
     return y, st[0], st[1]
 
@@ -376,6 +377,8 @@ def _ln_backward(dy, x, mean, rstd, weight, need, bias_dtype):
     C, dev = x.shape[-1], x.device
     w, _, pdt = _params(C, dev, weight, None)
     wdt = torch.float32 if w is None else w.dtype
+    if need[2] and bias_dtype is torch.float32 and wdt is not bias_dtype:     # (both gradients come in one type: the wider one)
+        w, wdt, pdt = w.float(), bias_dtype, _ffi.F32
     dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if need[0] else None
     dw = torch.empty(C, device=dev, dtype=wdt) if need[1] else None
     db = torch.empty(C, device=dev, dtype=wdt) if need[2] else None
@@ -388,6 +391,8 @@ def _ln_backward(dy, x, mean, rstd, weight, need, bias_dtype):
     rc = _launch(dev, lib.ydet_layer_norm_backward, d, _ptr(ws), nbytes)
     if rc:
         _ffi.check(rc, "ydet_layer_norm_backward")
+    if dw is not None and weight is not None and weight.dtype != wdt:
+        dw = dw.to(weight.dtype)
     if db is not None and bias_dtype is not None and bias_dtype != wdt:
         db = db.to(bias_dtype)
     return dx, dw, db
