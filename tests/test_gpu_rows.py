@@ -736,6 +736,22 @@ def test_gradients_of_parameters_of_two_types(wdt, bdt):
         assert ((got.double() - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("M,K,N", [(3, 64, 40), (900, 130, 40), (257, 64, 1000), (6400, 1030, 520), (23104, 2050, 500)])
+def test_weights_padded_further_than_needed(M, K, N):
+    # zeros behind K up to a pitch of the caller's choice; the rows of x end with their memory
+    g = gen(M)
+    q, s, wq, ws, bias = operands(g, M, K, N)
+    lin = ops.LinearI8(wq, ws, bias)
+    want = ops.matmul_i8(q, s, lin)
+    lin.kp += 448
+    wide = torch.zeros(lin.n_pad, lin.kp, device=DEV, dtype=torch.int8)
+    wide[:N, :K] = wq
+    lin.w = wide
+    assert torch.equal(ops.matmul_i8(q, s, lin), want)
+    x = randn(g, M, K)
+    assert torch.equal(ops.linear_i8(x, lin), ops.matmul_i8(*ops.quantize_rows(x), lin, out_dtype=F32))
+
+
 def test_second_derivative_is_an_error():
     x = torch.randn(4, 24, device=DEV, requires_grad=True)
     w = torch.randn(24, device=DEV, requires_grad=True)

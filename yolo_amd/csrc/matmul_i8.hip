@@ -161,7 +161,7 @@ __global__ __launch_bounds__(64 * WAVES_N * WAVES_M, 2) void tile_kernel(const A
                                                                         (int)(w_span < cap ? (unsigned)w_span : cap), 0x00020000);
     const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(a.x + m0 * a.x_ld), 0,
                                                                         (int)(x_span < cap ? (unsigned)x_span : cap), 0x00020000);
-    const int halves = a.kp / 64, nk = (halves + 1) / 2;
+    const int halves = (a.K + 63) / 64, nk = (halves + 1) / 2;
     unsigned ow[LW], ox[LX];
 #pragma unroll
     for (int j = 0; j < LW; ++j) {
@@ -192,7 +192,7 @@ __global__ __launch_bounds__(64 * WAVES_N * WAVES_M, 2) void tile_kernel(const A
             else __builtin_amdgcn_raw_ptr_buffer_load_lds(rr, dst, 4, ((k - 2 * BN / 64) * 64 + lane) * 4, 0, 0, 0);
         }
     }
-    // (kt's part may ride in the scalar offset: it lies below every extent, of at least one row's K and of one channel's kp)
+    // (kt's part may ride in the scalar offset: below K, it lies below every extent, of at least one row's K and of one channel's kp)
     auto issue = [&](int stage, int kt) {
         kt *= RB;
         char* dst = stages + stage * STAGE + wave * 1024;
@@ -395,7 +395,7 @@ __global__ __launch_bounds__(64 * NW) void few_rows_kernel(const Args a) {
     for (int i = 0; i < FN; ++i)
 #pragma unroll
         for (int j = 0; j < FM; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
-    const int steps = a.kp / 64;
+    const int steps = (a.K + 63) / 64;
     for (int s0 = wave; s0 < steps; s0 += NW * AHEAD) {
         i32x4 fa[AHEAD][FN], fb[AHEAD][FM];
 #pragma unroll
@@ -435,7 +435,7 @@ __global__ __launch_bounds__(512) void few_float_rows_kernel(const Args a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, p = lane & 15;
     const unsigned t = xcd_remap(blockIdx.x, gridDim.x);
     const int n0 = (int)(t % (unsigned)a.tiles_n) * 16, m0 = (int)(t / (unsigned)a.tiles_n) * 16;
-    const int steps = a.kp / 64, m = m0 + p < a.M ? m0 + p : a.M - 1;
+    const int steps = (a.K + 63) / 64, m = m0 + p < a.M ? m0 + p : a.M - 1;
     // Every load is made, pieces behind K from a page of zeros, so that all are in flight together.  RAG: the piece that holds the row's
     // end also holds what follows it, cleared below; behind the last row it is read value by value.
     typename P::type raw[AHEAD][NV];
@@ -502,7 +502,7 @@ __global__ __launch_bounds__(512) void few_float_rows_kernel(const Args a) {
 template <typename OUT, int BN, int BM, int WAVES_N, int WAVES_M, int NST = 2>
 static int launch_tile(Args a, hipStream_t stream) {
     constexpr int scales = (2 * BN + BM) * 4, stage = (BN + BM) * 128, most = scales + NST * stage;
-    const int used = (a.kp + 127) / 128, lds = scales + (used < NST ? used : NST) * stage;      // (fewer stages leave room for more workgroups)
+    const int used = (a.K + 127) / 128, lds = scales + (used < NST ? used : NST) * stage;      // (fewer stages leave room for more workgroups)
     a.tiles_n = (a.N + BN - 1) / BN;
     const long long blocks = (long long)a.tiles_n * ((a.M + BM - 1) / BM);
     YDET_CHECK_ARG(blocks * 64 * WAVES_N * WAVES_M <= UINT32_MAX, "matmul_i8: %d rows x %d channels are too many tiles", a.M, a.N);
