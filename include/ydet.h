@@ -527,10 +527,11 @@ int ydet_quantize_rows_i8(const ydet_quantize_desc* d, void* stream);
  *   y[r, n]   = act(acc * x_scale[r] * w_scale[n] + bias[n])  with the residual as in ydet_conv2d_nhwc (res_mode; res has y's dtype)
  * (in fp32 from the left: acc * x_scale[r] has to stay finite).
  * w [n_pad][kp], rows >= N and columns >= K zero, n_pad a multiple of 128, kp a multiple of 64; w_scale and bias (may be NULL)
- * hold n_pad values; all three 16-byte aligned.  Slices that are 16-byte aligned with x_ld a multiple of 16 are read in
- * 16-byte pieces (the bytes behind K in a row's last piece are read, their values do not matter; the slice's row has to hold
- * them); x may lie anywhere else too, and then many rows need ydet_matmul_i8_workspace_bytes(d) bytes of workspace (16-byte
- * aligned; 0: none, also for a descriptor that ydet_matmul_i8 refuses).  y may be res.  x_ld <= 2^23, rows < 2^31 - 512. */
+ * hold n_pad values; all three 16-byte aligned.  Slices that are 16-byte aligned with x_ld a multiple of 16 may be read in
+ * 16-byte pieces (the bytes behind K in a row's last piece are read, their values do not matter) if the slice's row holds
+ * them; x may lie anywhere else too, and where its address or x_ld is no multiple of 4, many rows need
+ * ydet_matmul_i8_workspace_bytes(d) bytes of workspace (16-byte aligned; 0: none, also for a descriptor that ydet_matmul_i8
+ * refuses).  y may be res.  x_ld <= 2^23, rows < 2^31 - 512. */
 typedef struct {
     const int8_t* x;
     const float* x_scale;

@@ -752,6 +752,22 @@ def test_weights_padded_further_than_needed(M, K, N):
     assert torch.equal(ops.linear_i8(x, lin), ops.matmul_i8(*ops.quantize_rows(x), lin, out_dtype=F32))
 
 
+@pytest.mark.parametrize("M,K,N", [(900, 77, 40), (700, 1000, 255), (3000, 1001, 130), (6400, 1030, 520), (23104, 2050, 500), (40000, 66, 64)])
+def test_rows_at_any_word(M, K, N):
+    """8-bit rows at 4-byte addresses and pitches, the last one at the very end of its memory (every tile, with and without a
+    whole word at the rows' end); the values between the rows do not matter."""
+    g = gen(M + K)
+    q, s, wq, ws, bias = operands(g, M, K, N)
+    lin = ops.LinearI8(wq, ws, bias)
+    want, e = product64(q, s, wq, ws, bias, "none", 0.1, None, "after")
+    k4 = (K + 3) // 4 * 4
+    for pitch, off in ((k4, 0), (k4 + 4, 4), (k4 + 44, 12), (K, 0), (K, 1)):
+        flat = torch.randint(-127, 128, ((M - 1) * pitch + off + K,), generator=g, device=DEV, dtype=torch.int8)
+        v = flat.as_strided((M, K), (pitch, 1), off)
+        v.copy_(q)
+        within(ops.matmul_i8(v, s, lin, out_dtype=F32), want, e + half(F32) * (want.abs() + e) + 1e-37)
+
+
 def test_second_derivative_is_an_error():
     x = torch.randn(4, 24, device=DEV, requires_grad=True)
     w = torch.randn(24, device=DEV, requires_grad=True)

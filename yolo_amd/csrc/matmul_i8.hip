@@ -137,8 +137,8 @@ __device__ __forceinline__ void load_channels(const float* ws, const float* bias
 // ---- tiles: BN channels x BM pixels, operands through LDS --------------------------------------------------------------
 // LDS image of a stage: BN weight rows, then BM pixel rows, 128 bytes of K each; row r's 16-byte piece c lies at place
 // c ^ ((r >> 1) & 7), so that the 16 rows a fragment read touches fall into 16 different places of the banks.  Stages are filled by
-// LDS-DMA (eight rows an instruction); rows behind the last pixel and channels behind n_pad lie outside the buffer
-// descriptors and read as zeros.  NST stages; the fragments of a half stage are read while the previous half's MFMAs run.
+// LDS-DMA (eight rows an instruction), from rows at any 4-byte address and pitch; rows behind the last pixel and channels behind
+// n_pad lie outside the buffer descriptors, which are checked word by word, and read as zeros.  NST stages; the fragments of a half stage are read while the previous half's MFMAs run.
 // What bounds it: for long K the operands' way through L2 (52 us for 23104 x 4096 -> 512 with 256 x 192 tiles: 1.85 POP/s, where a
 // library product of 8192^3 reaches 2.06), for short K the rows and the output (52 us for 409600 x 128 -> 128 with SiLU and
 // residual: 5.0 TB/s), for many channels and short K the epilogue, about ten operations a value, two of them transcendental
@@ -155,7 +155,7 @@ __global__ __launch_bounds__(64 * WAVES_N * WAVES_M, 2) void tile_kernel(const A
     const unsigned t = xcd_remap(blockIdx.x, gridDim.x);
     const int n0 = (int)(t % (unsigned)a.tiles_n) * BN, m0 = (int)(t / (unsigned)a.tiles_n) * BM;
 
-    const long long w_span = (long long)(a.n_pad - n0) * a.kp, x_span = (long long)(a.M - 1 - m0) * a.x_ld + ((a.K + 15) & ~15);
+    const long long w_span = (long long)(a.n_pad - n0) * a.kp, x_span = (long long)(a.M - 1 - m0) * a.x_ld + ((a.K + 3) & ~3);
     const unsigned cap = 0xffffffffu;
     const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(a.w + (long long)n0 * a.kp), 0,
                                                                         (int)(w_span < cap ? (unsigned)w_span : cap), 0x00020000);
@@ -555,7 +555,8 @@ __global__ __launch_bounds__(256) void align_rows_kernel(const char* x, long lon
 //     eight 13.6);
 //   64 x 128 otherwise (409600 x 64 -> 64: 18, in 128 x 128 tiles 28; 409600 x 128 -> 128 with residual: 52 against 62), with a
 //     third stage where there are fewer than two workgroups a CU (2888 x 4096 -> 512: 14.6, with two stages 19.2).
-// The tile kernels want rows in 16-byte pieces: others are first copied into the workspace.
+// The tile kernels want rows at 4-byte addresses and pitches: others are first copied into the workspace (2888 x 1000 -> 255: 3.4 us
+// and a launch more on top of 6.8).
 static long long tiles(const Args& a, int bn, int bm) { return (long long)((a.N + bn - 1) / bn) * ((a.M + bm - 1) / bm); }
 static int direct_size(const Args& a) {
     const int cus = current_device_info().cus;
@@ -587,8 +588,12 @@ static int launch(const Args& a, bool wide_x, hipStream_t stream) {
 
 using namespace ydet;
 
-// Checks a descriptor and fills the launch arguments; wide_x: its rows can be read in 16-byte pieces.
-static int fill_args(const ydet_matmul_i8_desc* d, i8::Args& a, bool& wide_x) {
+// How the rows of x lie: at any byte, in whole words (for LDS-DMA), or in 16-byte pieces (for plain loads) that may reach
+// behind K, so that the pitch has to hold them.
+enum class Rows { bytes, words, pieces };
+
+// Checks a descriptor and fills the launch arguments.
+static int fill_args(const ydet_matmul_i8_desc* d, i8::Args& a, Rows& lie) {
     YDET_CHECK_ARG(d, "matmul_i8: null descriptor");
     YDET_CHECK_ARG(d->rows >= 0 && d->rows <= INT32_MAX - 512 && d->K > 0 && d->K <= 131071 && d->N > 0 && d->N <= (1 << 24),
                    "matmul_i8: rows=%lld K=%d N=%d (K up to 131071: the sums are 32-bit integers)", (long long)d->rows, d->K, d->N);
@@ -614,8 +619,8 @@ static int fill_args(const ydet_matmul_i8_desc* d, i8::Args& a, bool& wide_x) {
     YDET_CHECK_ARG(((uintptr_t)a.y | (uintptr_t)a.res) % es == 0 && (uintptr_t)a.xs % 4 == 0, "matmul_i8: misaligned tensor");
     a.M = (int)d->rows, a.K = d->K, a.N = d->N, a.kp = d->kp, a.n_pad = d->n_pad;
     a.x_ld = d->x_ld, a.y_ld = d->y_ld, a.res_ld = d->res_ld, a.act = d->act, a.slope = d->act == YDET_ACT_LEAKY ? d->slope : 1.f;
-    // (the last piece of a row may reach behind K, so the pitch has to hold it)
-    wide_x = (uintptr_t)a.x % 16 == 0 && d->x_ld % 16 == 0 && d->x_coff + (d->K + 15) / 16 * 16 <= d->x_ld;
+    const uintptr_t at = (uintptr_t)a.x | (uintptr_t)(unsigned)d->x_ld;
+    lie = at % 16 == 0 && d->x_coff + (d->K + 15) / 16 * 16 <= d->x_ld ? Rows::pieces : at % 4 == 0 ? Rows::words : Rows::bytes;
     return YDET_OK;
 }
 
@@ -623,10 +628,10 @@ static size_t aligned_bytes(const i8::Args& a) { return (size_t)a.M * ((a.K + 15
 
 int ydet_launch_matmul_i8(const ydet_matmul_i8_desc* d, void* ws, size_t ws_bytes, hipStream_t stream) {
     i8::Args a;
-    bool wide_x;
-    const int rc = fill_args(d, a, wide_x);
+    Rows lie;
+    const int rc = fill_args(d, a, lie);
     if (rc != YDET_OK || a.M == 0) return rc;
-    if (!wide_x && !i8::direct_size(a)) {
+    if (lie == Rows::bytes && !i8::direct_size(a)) {
         if (ws_bytes < aligned_bytes(a))
             return fail(YDET_ERR_WORKSPACE, "matmul_i8: workspace %zu < %zu bytes", ws_bytes, aligned_bytes(a));
         YDET_CHECK_ARG(ws && (uintptr_t)ws % 16 == 0, "matmul_i8: rows of %d at this address and pitch need a 16-byte aligned workspace", a.K);
@@ -634,16 +639,17 @@ int ydet_launch_matmul_i8(const ydet_matmul_i8_desc* d, void* ws, size_t ws_byte
         hipLaunchKernelGGL(i8::align_rows_kernel, dim3((unsigned)(blocks < (1 << 20) ? blocks : (1 << 20))), dim3(256), 0, stream, a.x, a.x_ld, a.M,
                            a.K, static_cast<char*>(ws));
         YDET_CHECK_LAUNCH("matmul_i8 (rows)");
-        a.x = static_cast<const char*>(ws), a.x_ld = (a.K + 15) / 16 * 16, wide_x = true;
+        a.x = static_cast<const char*>(ws), a.x_ld = (a.K + 15) / 16 * 16;
     }
+    const bool wide_x = lie == Rows::pieces;
     return d->out_dtype == YDET_BF16 ? i8::launch<__bf16>(a, wide_x, stream) : i8::launch<float>(a, wide_x, stream);
 }
 
 extern "C" size_t ydet_matmul_i8_workspace_bytes(const ydet_matmul_i8_desc* d) {
     clear_error();
     i8::Args a;
-    bool wide_x;
-    if (fill_args(d, a, wide_x) != YDET_OK || wide_x || a.M == 0 || i8::direct_size(a)) return 0;
+    Rows lie;
+    if (fill_args(d, a, lie) != YDET_OK || lie != Rows::bytes || a.M == 0 || i8::direct_size(a)) return 0;
     return aligned_bytes(a);
 }
 
@@ -660,8 +666,8 @@ static int fill_linear(const ydet_quantize_desc* in, const ydet_matmul_i8_desc* 
     q.q_ld = p.x_ld = (in->C + 15) / 16 * 16, p.x_coff = 0;
     p.x = q.q = static_cast<int8_t*>(at);
     p.x_scale = q.scale = reinterpret_cast<float*>(q.q + in->rows * q.q_ld);
-    bool wide_x;
-    return fill_args(&p, a, wide_x);
+    Rows lie;
+    return fill_args(&p, a, lie);
 }
 
 static bool fused(const ydet_quantize_desc& q, const i8::Args& a) { return !q.normalize && i8::fuses(a); }

@@ -567,7 +567,7 @@ def matmul_i8(q, scale, lin, act="none", slope=0.1, res=None, res_mode="after", 
     y, d, keep = _product(q.data_ptr(), scale.data_ptr(), n, ld, lin, act, slope, res, res_mode, out_dtype)
     lib = _ffi.lib()
     ws, nbytes = None, 0
-    if ld % 16 or d.x % 16:
+    if ld % 4 or d.x % 4:
         nbytes = lib.ydet_matmul_i8_workspace_bytes(d)
         ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
     rc = _launch(dev, lib.ydet_matmul_i8, d, _ptr(ws), nbytes)
