@@ -290,7 +290,7 @@ MAX_ROW = 8192      # channels of a row that layer_norm and quantize_rows take
 def _launch(dev, call, *args):
     """`call(*args, stream)` on torch's current stream of `dev`."""
     i = dev.index
-    if torch.cuda.current_device() == i:
+    if torch._C._cuda_getDevice() == i:
         return call(*args, torch._C._cuda_getCurrentRawStream(i))
     with torch.cuda.device(i):
         return call(*args, torch._C._cuda_getCurrentRawStream(i))
@@ -318,9 +318,10 @@ def _as_rows(t, what):
 def _params(C, dev, w, b):
     """The per-channel parameters (None allowed) as contiguous tensors of one type, and that type."""
     td = None
+    want = (C,)
     for p in (w, b):
         if p is not None:
-            if p.shape != (C,):
+            if p.shape != want:
                 raise ValueError(f"weight and bias have one value a channel: got {tuple(p.shape)} for {C} channels")
             if p.device != dev:
                 raise RuntimeError(f"weight / bias on {p.device}, the input on {dev}")
@@ -346,10 +347,10 @@ def _ln_forward(x, weight, bias, eps, stats):
     x, n, ld = _as_rows(x, "layer_norm")
     C, dev = x.shape[-1], x.device
     w, b, pdt = _params(C, dev, weight, bias)
-    y = torch.empty(x.shape, device=dev, dtype=x.dtype)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     st = mean = rstd = None
     if stats:
-        st = torch.empty((2,) + x.shape[:-1], device=dev, dtype=torch.float32)
+        st = x.new_empty((2,) + x.shape[:-1], dtype=torch.float32)
         mean = st.data_ptr()
         rstd = mean + 4 * n
     d = _ffi.LayerNormDesc(x.data_ptr(), y.data_ptr(), w if w is None else w.data_ptr(), b if b is None else b.data_ptr(), mean, rstd,
@@ -379,13 +380,13 @@ def _ln_backward(dy, x, mean, rstd, weight, need, bias_dtype):
     wdt = torch.float32 if w is None else w.dtype
     if need[2] and bias_dtype is torch.float32 and wdt is not bias_dtype:     # (both gradients come in one type: the wider one)
         w, wdt, pdt = w.float(), bias_dtype, _ffi.F32
-    dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if need[0] else None
-    dw = torch.empty(C, device=dev, dtype=wdt) if need[1] else None
-    db = torch.empty(C, device=dev, dtype=wdt) if need[2] else None
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need[0] else None
+    dw = x.new_empty(C, dtype=wdt) if need[1] else None
+    db = x.new_empty(C, dtype=wdt) if need[2] else None
     ws, nbytes = None, 0
     if need[1] or need[2]:
         nbytes = lib.ydet_layer_norm_backward_workspace_bytes(n, C)
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        ws = x.new_empty(nbytes, dtype=torch.uint8)
     d = _ffi.LayerNormGradDesc(dy.data_ptr(), x.data_ptr(), _ptr(dx), _ptr(w), mean, rstd, _ptr(dw), _ptr(db),
                                n, C, dy_ld, 0, ld, 0, C, 0, dt, pdt)
     rc = _launch(dev, lib.ydet_layer_norm_backward, d, _ptr(ws), nbytes)
@@ -455,13 +456,13 @@ def _quantize(x, normalize, weight, bias, eps):
     C, dev, lead = x.shape[-1], x.device, x.shape[:-1]
     w, b, pdt = _params(C, dev, weight, bias)
     q_ld = (C + 15) // 16 * 16
-    q = torch.empty(lead + (q_ld,), device=dev, dtype=torch.int8)
-    scale = torch.empty(lead, device=dev, dtype=torch.float32)
+    q = x.new_empty(*lead, q_ld, dtype=torch.int8)
+    scale = x.new_empty(n, dtype=torch.float32)
     d = _ffi.QuantizeDesc(x.data_ptr(), q.data_ptr(), scale.data_ptr(), _ptr(w), _ptr(b), n, C, ld, 0, q_ld, dt, pdt, normalize, eps)
     rc = _launch(dev, _ffi.lib().ydet_quantize_rows_i8, d)
     if rc:
         _ffi.check(rc, "ydet_quantize_rows_i8")
-    return (q if q_ld == C else q[..., :C]), scale
+    return (q if q_ld == C else q[..., :C]), (scale if len(lead) == 1 else scale.view(lead))
 
 
 def quantize_rows(x):
@@ -536,7 +537,7 @@ def _product(x, scale, n, ld, lin, act, slope, res, res_mode, out_dtype):
             raise RuntimeError(f"res on {res.device}, the weights on {dev}")
         res, _, r_ld = _as_rows(res, "matmul_i8")
         rmode, rptr = _RES[res_mode], res.data_ptr()
-    y = torch.empty((n, N), device=dev, dtype=out_dtype)
+    y = lin.w.new_empty(n, N, dtype=out_dtype)
     return y, _ffi.MatmulI8Desc(x, scale, lin.w.data_ptr(), lin.scale.data_ptr(), _ptr(lin.bias), rptr, y.data_ptr(), n, lin.K, N, lin.kp,
                                 lin.n_pad, ld, 0, N, 0, r_ld, 0, _ACTS[act], slope, rmode, odt), res
 
@@ -569,7 +570,7 @@ def matmul_i8(q, scale, lin, act="none", slope=0.1, res=None, res_mode="after", 
     ws, nbytes = None, 0
     if ld % 4 or d.x % 4:
         nbytes = lib.ydet_matmul_i8_workspace_bytes(d)
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+        ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     rc = _launch(dev, lib.ydet_matmul_i8, d, _ptr(ws), nbytes)
     if rc:
         _ffi.check(rc, "ydet_matmul_i8")
@@ -595,7 +596,7 @@ def linear_i8(x, lin, act="none", slope=0.1, res=None, res_mode="after", out_dty
     y, d, keep = _product(None, None, n, 0, lin, act, slope, res, res_mode, x.dtype if out_dtype is None else out_dtype)
     src = _ffi.QuantizeDesc(x.data_ptr(), None, None, None, None, n, K, ld, 0, 0, dt, _ffi.F32, 0, 0.0)
     nbytes = lib.ydet_linear_i8_workspace_bytes(src, d)
-    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     rc = _launch(dev, lib.ydet_linear_i8, src, d, _ptr(ws), nbytes)
     if rc:
         _ffi.check(rc, "ydet_linear_i8")
