@@ -180,8 +180,8 @@ __global__ __launch_bounds__(kThreads) void row_norm_kernel(const RowArgs a) {
 }
 
 // Workgroups: each walks over rows, weight and bias in its registers.  No more than stay resident where a workgroup reads weight and
-// bias (23104 x 2048 norm + quantisation in bf16: 54 us with four a CU, 72 with one for every four rows; rows of up to 1024
-// values have room for eight a CU), twice as many where it reads none (25600 x 512 quantisation: 10.9 us, with eight 11.6) or
+// bias (23104 x 2048 norm + quantisation in bf16, 64 lanes a row: 54 us with four a CU, 72 with one for every four rows; up to 16
+// values a lane leave room for eight a CU), twice as many where it reads none (25600 x 512 quantisation: 10.9 us, with eight 11.6) or
 // takes four rows at a time (409600 x 128 norm: 39.2 us, with eight 41.7).
 template <int MODE, typename T, bool RAG, int LPR, int CH, int RPT>
 static int launch_rows(const RowArgs& a, hipStream_t stream) {
@@ -196,23 +196,26 @@ static int launch_rows(const RowArgs& a, hipStream_t stream) {
 // one where the rows are quantised (four cost 148 registers: 102400 x 256 norm + quantisation 28.2 us, with one 20.4).
 template <int MODE, typename T, bool RAG, int LPR, int CH>
 static int launch_depth(const RowArgs& a, hipStream_t stream) {
-    if constexpr (CH == 1 && !(MODE & kQuant)) {
+    if constexpr (CH == 1 && LPR <= 64 && !(MODE & kQuant)) {
         if (a.rows >= (long long)current_device_info().cus * 8 * 4 * (kThreads / LPR))
             return launch_rows<MODE, T, RAG, LPR, CH, 4>(a, stream);
     }
     return launch_rows<MODE, T, RAG, LPR, CH, 1>(a, stream);
 }
 
+// Longer rows take a whole workgroup: fewer values, weights and biases a lane leave room for more waves (norm + quantisation of
+// 23104 x 2048 in bf16 41 us, inside a wave 54; of 400 x 1200 4.7 and 7.3; norm of 5000 x 1500 in fp32 12.2 and 14.5).
+constexpr int kWaveCols = 1024;
 template <int MODE, typename T, bool RAG>
 static int launch_shape(const RowArgs& a, hipStream_t stream) {
-    const Shape s = shape_of(a.cw, 16 / (int)sizeof(T));
+    const Shape s = shape_of(a.cw, 16 / (int)sizeof(T), kWaveCols);
 #define YDET_ROWS(L, K) \
     if (s.lpr == L && s.ch == K) return launch_depth<MODE, T, RAG, L, K>(a, stream);
-    YDET_ROWS(4, 1) YDET_ROWS(8, 1) YDET_ROWS(16, 1) YDET_ROWS(32, 1) YDET_ROWS(64, 1) YDET_ROWS(64, 2) YDET_ROWS(64, 4) YDET_ROWS(256, 4)
+    YDET_ROWS(4, 1) YDET_ROWS(8, 1) YDET_ROWS(16, 1) YDET_ROWS(32, 1) YDET_ROWS(64, 1) YDET_ROWS(64, 2) YDET_ROWS(256, 2) YDET_ROWS(256, 4)
     if constexpr (sizeof(T) == 4) {
-        YDET_ROWS(64, 8) YDET_ROWS(256, 8)
+        YDET_ROWS(64, 4) YDET_ROWS(256, 8)
     } else {
-        YDET_ROWS(256, 2)
+        YDET_ROWS(256, 1)
     }
 #undef YDET_ROWS
     return fail(YDET_ERR_ARG, "row norm: no kernel for %d channels", a.C);

@@ -6,8 +6,7 @@ namespace ydet {
 namespace rows {
 
 // A row of C values is held in registers by LPR lanes (a power of two: a part of a wave, a wave, or the 256 lanes of a
-// workgroup), CH pieces of VEC values each; piece c of lane l starts at column (c * LPR + l) * VEC.  At most 32 values a lane:
-// rows up to 2048 values stay inside one wave, up to kMaxC inside one workgroup.
+// workgroup), CH pieces of VEC values each; piece c of lane l starts at column (c * LPR + l) * VEC.  At most 32 values a lane.
 constexpr int kMaxC = 8192;
 constexpr int kThreads = 256;
 
@@ -19,16 +18,14 @@ static inline int pow2_at_least(int v) {
     while (p < v) p *= 2;
     return p;
 }
-// cols: values of a row that are read or written; vec: values of a 16-byte piece (8 or 4)
-static inline Shape shape_of(int cols, int vec) {
+// cols: values of a row that are read or written; vec: values of a 16-byte piece (8 or 4); rows up to wave_cols stay inside a wave
+static inline Shape shape_of(int cols, int vec, int wave_cols) {
     const int n = (cols + vec - 1) / vec;
     if (n <= 64) {
         const int l = pow2_at_least(n);
         return Shape{l < 4 ? 4 : l, 1};
     }
-    if (n * vec <= 2048) return Shape{64, pow2_at_least((n + 63) / 64)};
-    const int least = vec == 4 ? 4 : 2, c = pow2_at_least((n + 255) / 256);
-    return Shape{256, c < least ? least : c};
+    return n * vec <= wave_cols ? Shape{64, pow2_at_least((n + 63) / 64)} : Shape{256, pow2_at_least((n + 255) / 256)};
 }
 
 template <int CTRL>
