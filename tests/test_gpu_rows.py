@@ -877,3 +877,16 @@ def test_in_place():
                           lin.n_pad, q.stride(0), 0, 40, 0, 40, 0, _ffi.ACT_SILU, 0.0, _ffi.RES_AFTER_ACT, _ffi.BF16)
     _ffi.check(lib.ydet_matmul_i8(d, None, 0, st))
     assert torch.equal(x3, want)
+
+
+@pytest.mark.parametrize("K", [30, 32, 64])
+@pytest.mark.parametrize("lead", [(0,), (3, 0), (0, 5)])
+def test_empty_batches_through_a_block(lead, K):
+    """Norm, 8 bits and products of a batch without rows, at row pitches that are and are not multiples of 4."""
+    lin = ops.LinearI8.quantize(torch.randn(20, K, device=DEV))
+    x = torch.empty(*lead, K, device=DEV, dtype=BF16)
+    q, s = ops.layer_norm_quantize(x, torch.ones(K, device=DEV))
+    assert q.shape == lead + (K,) and s.shape == lead
+    y = ops.matmul_i8(q, s, lin, act="silu", res=torch.empty(*lead, 20, device=DEV, dtype=BF16))
+    assert y.shape == lead + (20,) and y.dtype == BF16
+    assert ops.matmul_i8(*ops.quantize_rows(x), lin, out_dtype=F32).shape == ops.linear_i8(x, lin).shape == lead + (20,)

@@ -165,3 +165,26 @@ def test_which_layers_go_to_8_bits():
     finally:
         engine.set_pointwise_int8(False)
     assert not any(k == "linear_i8" for k, _ in plan.g.ops) and plan.i8_ws == [None]
+
+
+# ---- batches without rows: nothing is launched, so the wrappers run here up to the library's own return -----------------------
+@pytest.fixture
+def without_gpu(monkeypatch):
+    monkeypatch.setattr(ops, "_need_cuda", lambda *t: None)
+    monkeypatch.setattr(ops, "_launch", lambda dev, call, *args: call(*args, None))
+
+
+@pytest.mark.parametrize("lead", [(0,), (3, 0), (0, 5)])
+@pytest.mark.parametrize("K", [30, 32, 64, 77, 1024])
+def test_products_without_rows(without_gpu, K, lead):
+    """Whatever the rows' pitch (a multiple of 4 or not): an empty output of the right shape."""
+    lin = ops.LinearI8(torch.ones(20, K, dtype=torch.int8), torch.ones(20), torch.ones(20))
+    x = torch.empty(*lead, K)
+    q, s = ops.quantize_rows(x)
+    assert q.shape == lead + (K,) and s.shape == lead
+    for rows in (q, torch.empty(*lead, K, dtype=torch.int8)):
+        y = ops.matmul_i8(rows, s, lin, act="silu")
+        assert y.shape == lead + (20,) and y.dtype == torch.bfloat16
+        assert ops.matmul_i8(rows, s, lin, res=torch.empty(*lead, 20), out_dtype=torch.float32).shape == lead + (20,)
+    assert ops.matmul_i8(*ops.layer_norm_quantize(x), lin).shape == lead + (20,)
+    assert ops.linear_i8(x, lin).shape == lead + (20,)

@@ -565,10 +565,11 @@ def matmul_i8(q, scale, lin, act="none", slope=0.1, res=None, res_mode="after", 
         q, ld = q.clone(memory_format=torch.contiguous_format), K
     if not scale.is_contiguous():
         scale = scale.contiguous()
-    y, d, keep = _product(q.data_ptr(), scale.data_ptr(), n, ld, lin, act, slope, res, res_mode, out_dtype)
+    at = q.data_ptr()       # (0 without rows)
+    y, d, keep = _product(at, scale.data_ptr(), n, ld, lin, act, slope, res, res_mode, out_dtype)
     lib = _ffi.lib()
     ws, nbytes = None, 0
-    if ld % 4 or d.x % 4:
+    if (ld | at) % 4:
         nbytes = lib.ydet_matmul_i8_workspace_bytes(d)
         ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     rc = _launch(dev, lib.ydet_matmul_i8, d, _ptr(ws), nbytes)
