@@ -531,7 +531,7 @@ int ydet_quantize_rows_i8(const ydet_quantize_desc* d, void* stream);
  * 16-byte pieces (the bytes behind K in a row's last piece are read, their values do not matter) if the slice's row holds
  * them; x may lie anywhere else too, and where its address or x_ld is no multiple of 4, many rows need
  * ydet_matmul_i8_workspace_bytes(d) bytes of workspace (16-byte aligned; 0: none, also for a descriptor that ydet_matmul_i8
- * refuses).  y may be res.  x_ld <= 2^23, rows < 2^31 - 512. */
+ * refuses).  y may be res; y and x do not overlap.  x_ld <= 2^23, rows < 2^31 - 512. */
 typedef struct {
     const int8_t* x;
     const float* x_scale;
@@ -554,7 +554,8 @@ int ydet_matmul_i8(const ydet_matmul_i8_desc* d, void* workspace, size_t workspa
 /* ydet_quantize_rows_i8 (normalize included) and ydet_matmul_i8 behind each other, with the same result: `in` without q, scale
  * and q_ld, `product` without x, x_scale, x_ld and x_coff; in->rows == product->rows, in->C == product->K.  Few rows take one
  * launch; otherwise the 8-bit rows go to the caller's workspace (ydet_linear_i8_workspace_bytes, 16-byte aligned; 0: none,
- * also for a pair that ydet_linear_i8 refuses). */
+ * also for a pair that ydet_linear_i8 refuses).  y may overlap in->x in any way (y == res == in->x: a block in place) where
+ * there is a workspace of rows * (C rounded up to 16) + 16 * ceil(rows / 4) bytes; few rows without one are refused then. */
 size_t ydet_linear_i8_workspace_bytes(const ydet_quantize_desc* in, const ydet_matmul_i8_desc* product);
 int ydet_linear_i8(const ydet_quantize_desc* in, const ydet_matmul_i8_desc* product, void* workspace, size_t workspace_bytes,
                    void* stream);

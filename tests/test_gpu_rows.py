@@ -890,3 +890,26 @@ def test_empty_batches_through_a_block(lead, K):
     y = ops.matmul_i8(q, s, lin, act="silu", res=torch.empty(*lead, 20, device=DEV, dtype=BF16))
     assert y.shape == lead + (20,) and y.dtype == BF16
     assert ops.matmul_i8(*ops.quantize_rows(x), lin, out_dtype=F32).shape == ops.linear_i8(x, lin).shape == lead + (20,)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M,K,N", [(1, 64, 64), (40, 512, 512), (100, 256, 256), (33, 200, 90), (900, 128, 128), (5000, 96, 96)])
+def test_linear_in_place(M, K, N, dtype):
+    """The output over the floating rows it is made from (and over the residual), few rows and many: the bits of the call apart,
+    given a workspace; few rows without one are refused."""
+    g = gen(M + K)
+    lib, st = _ffi.lib(), _ffi.current_stream()
+    x = randn(g, M, K, dtype=dtype)
+    lin = ops.LinearI8.quantize(randn(g, N, K) / math.sqrt(K), randn(g, N))
+    shortcut = N == K
+    want = ops.linear_i8(x, lin, act="silu", res=x if shortcut else None)
+    dt = ops._dt(x)
+    at = x.clone()
+    q = _ffi.QuantizeDesc(at.data_ptr(), None, None, None, None, M, K, K, 0, 0, dt, _ffi.F32, 0, 0.0)
+    d = _ffi.MatmulI8Desc(None, None, lin.w.data_ptr(), lin.scale.data_ptr(), lin.bias.data_ptr(), at.data_ptr(), at.data_ptr(), M, K, N, lin.kp,
+                          lin.n_pad, 0, 0, K, 0, K, 0, _ffi.ACT_SILU, 0.0, _ffi.RES_AFTER_ACT if shortcut else _ffi.RES_NONE, dt)
+    assert lib.ydet_linear_i8(q, d, None, 0, st) < 0
+    nbytes = M * ((K + 15) // 16 * 16) + (M + 3) // 4 * 16
+    ws = torch.empty(nbytes, device=DEV, dtype=torch.uint8)
+    _ffi.check(lib.ydet_linear_i8(q, d, ws.data_ptr(), nbytes, st))
+    assert torch.equal(at[:, :N], want) and torch.equal(at[:, N:], x[:, N:])

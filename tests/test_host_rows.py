@@ -188,3 +188,35 @@ def test_products_without_rows(without_gpu, K, lead):
         assert ops.matmul_i8(rows, s, lin, res=torch.empty(*lead, 20), out_dtype=torch.float32).shape == lead + (20,)
     assert ops.matmul_i8(*ops.layer_norm_quantize(x), lin).shape == lead + (20,)
     assert ops.linear_i8(x, lin).shape == lead + (20,)
+
+
+def test_few_rows_in_place_need_a_workspace():
+    """An output over the floating rows never takes the one launch; beside them, also in the same rows, it does.  (A workspace that is
+    too small or misaligned says that two launches would be taken, a bad type of the rows that the one launch was reached: nothing is
+    launched here.)"""
+    lib = _ffi.lib()
+
+    def meets(rows=16, K=64, N=64, x=P, y=P, x_ld=64, y_ld=64, x_coff=0, y_coff=0, dtype=1, out=1):
+        q = _ffi.QuantizeDesc(x=x, rows=rows, C=K, x_ld=x_ld, x_coff=x_coff, dtype=dtype, param_dtype=7)
+        d = _ffi.MatmulI8Desc(w=P, w_scale=P, y=y, rows=rows, K=K, N=N, kp=(K + 63) // 64 * 64, n_pad=(N + 127) // 128 * 128, y_ld=y_ld,
+                              y_coff=y_coff, out_dtype=out)
+        bytes_ = rows * ((K + 15) // 16 * 16) + (rows + 3) // 4 * 16
+        rc = lib.ydet_linear_i8(q, d, P, bytes_ - 1, None)
+        text = lib.ydet_last_error().decode()
+        assert (rc == WS and f"{bytes_ - 1} < {bytes_}" in text) or (rc == ARG and "dtype" in text)
+        assert lib.ydet_linear_i8(q, d, None, 0, None) in (ARG, WS)
+        return rc == WS
+    assert meets()                                                          # in place
+    assert not meets(y=P + 16 * 128) and not meets(y=P - 16 * 128)          # behind and before
+    assert meets(y=P + 16 * 128 - 2) and meets(y=P - 16 * 128 + 2)          # over the last and the first value
+    for x0, y0, m in ((0, 64, False), (64, 0, False), (0, 63, True), (63, 0, True), (0, 0, True), (1, 65, False), (65, 1, False)):
+        assert meets(x_ld=129, y_ld=129, x_coff=x0, y_coff=y0) == m, (x0, y0)
+    wide = dict(x_ld=200, y_ld=200)
+    assert not meets(**wide, y=P + 3 * 400, y_coff=100)                     # other rows, other columns
+    assert not meets(**wide, y=P + 3 * 400, y_coff=180, N=20)
+    assert meets(**wide, x=P + 2 * 100, N=120)                              # (columns 0 .. 119 and 100 .. 163)
+    assert not meets(**wide, y=P + 2 * 180, N=20) and meets(**wide, y=P + 2 * 180, N=21)      # up to the next row of x, into it
+    assert meets(x_ld=128, y_ld=256, y_coff=64)                             # other pitches: their ranges meet
+    # other types of rows and output
+    assert not meets(dtype=0, out=1, x_ld=128, y_ld=256, y_coff=128) and meets(dtype=0, out=1, x_ld=128, y_ld=256, y_coff=127)
+    assert not meets(rows=1, y=P + 128) and meets(rows=1, y=P + 126)

@@ -670,6 +670,17 @@ static int fill_linear(const ydet_quantize_desc* in, const ydet_matmul_i8_desc* 
     return fill_args(&p, a, lie);
 }
 
+// Whether the output touches bytes of the floating rows.  Slices of one pitch that take different columns of it do not.
+static bool writes_input(const ydet_quantize_desc& q, const ydet_matmul_i8_desc& p) {
+    const long long xe = (long long)dtype_size(q.dtype), ye = (long long)dtype_size(p.out_dtype);
+    const long long x = (long long)(uintptr_t)q.x + q.x_coff * xe, y = (long long)(uintptr_t)p.y + p.y_coff * ye;
+    const long long x_row = q.C * xe, y_row = p.N * ye, x_ld = q.x_ld * xe, y_ld = p.y_ld * ye;
+    if (y + (p.rows - 1) * y_ld + y_row <= x || x + (q.rows - 1) * x_ld + x_row <= y) return false;
+    if (x_ld != y_ld) return true;
+    const long long at = ((y - x) % x_ld + x_ld) % x_ld;       // where in a row of x one of y begins
+    return at < x_row || at + y_row > x_ld;
+}
+
 static bool fused(const ydet_quantize_desc& q, const i8::Args& a) { return !q.normalize && i8::fuses(a); }
 
 static size_t linear_bytes(const ydet_quantize_desc& q) { return (size_t)q.rows * q.q_ld + (size_t)(q.rows + 3) / 4 * 16; }
@@ -689,7 +700,9 @@ int ydet_launch_linear_i8(const ydet_quantize_desc* in, const ydet_matmul_i8_des
     i8::Args a;
     int rc = fill_linear(in, product, ws ? ws : reinterpret_cast<void*>(256), q, p, a);
     if (rc != YDET_OK || q.rows == 0) return rc;
-    if (fused(q, a)) {
+    // (in one launch workgroups read whole rows while others already store their channels: not where those are the same bytes.  In
+    // two, every row is in 8 bits before the first store.)
+    if (fused(q, a) && !writes_input(q, p)) {
         rc = ydet_check_quantize_rows(&q);
         if (rc != YDET_OK) return rc;
         a.x = static_cast<const char*>(q.x) + q.x_coff * dtype_size(q.dtype), a.x_ld = q.x_ld, a.xs = nullptr;
