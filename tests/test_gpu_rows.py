@@ -913,3 +913,26 @@ def test_linear_in_place(M, K, N, dtype):
     ws = torch.empty(nbytes, device=DEV, dtype=torch.uint8)
     _ffi.check(lib.ydet_linear_i8(q, d, ws.data_ptr(), nbytes, st))
     assert torch.equal(at[:, :N], want) and torch.equal(at[:, N:], x[:, N:])
+
+
+def test_parameter_gradients_of_very_many_rows():
+    """The sums over rows keep their error however many there are: a lane adds at most 1024 rows one after the other, then come the
+    64 groups of a workgroup, 11 launches and a tree of 16.  (Equal terms of this value drift one way: a chain of all the rows of a
+    lane group, 10 681, ends 1.5e-4 off.)"""
+    rows, c = 700_000_001, 1.521
+    dy = torch.full((rows, 1), c, device=DEV)
+    x = torch.ones(rows, 1, device=DEV)
+    mean, rstd = torch.zeros(rows, device=DEV), torch.ones(rows, device=DEV)
+    _, dw, db = ops.layer_norm_backward(dy, x, mean, rstd, need=(False, True, True))
+    want = rows * float(torch.tensor(c, dtype=F32))
+    for got in (dw, db):
+        assert abs(float(got) - want) <= (1024 + 64 + 11 + 16) * U * want
+    # and every row is there once: rows and launches of unlike values
+    dy[:] = 0
+    marks = torch.tensor([0, 1, 63, 67_108_863, 67_108_864, 134_217_727, 500_000_000, rows - 1], device=DEV)
+    dy[marks, 0] = 2.0 ** torch.arange(8, device=DEV)
+    x[marks, 0] = 3.0
+    dx, dw, db = ops.layer_norm_backward(dy, x, mean, rstd)
+    assert float(db) == 255 and float(dw) == 3 * 255
+    # dx = r (g - g - xh g xh): with one channel and these statistics, -9 dy at the marks and nothing elsewhere
+    assert torch.equal(dx[marks, 0], -9 * dy[marks, 0]) and int((dx != 0).sum()) == 8

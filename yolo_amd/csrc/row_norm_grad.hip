@@ -5,8 +5,10 @@
 // One pass over dy and x serves all three: a row sits in the registers of the lanes that share it (rows_common.h), which take
 // its two sums and write dx, while every lane keeps running sums of dw and db for the columns it owns, over all rows it
 // meets.  A workgroup's lane groups then meet in LDS and leave one partial sum a column in the workspace, and a second kernel
-// adds the workgroups' partial sums in a fixed order: no atomics, the same bits every time.  All sums are in 32 bits, none longer
-// than the rows of a lane group (tens to hundreds) plus the tree over the groups and workgroups.  Bound by HBM: 6 bytes a bf16 value.
+// adds the workgroups' partial sums in a fixed order: no atomics, the same bits every time.  All sums are in 32 bits.  A lane adds
+// at most kChain rows one after the other; more rows than that for every lane group (1 M of more than 2048 bf16 channels, 67 M of
+// up to 16) take another launch, which adds to the partial sums.  Behind the lanes come at most 64 groups, one term a launch, and the
+// tree over the workgroups.  Bound by HBM: 6 bytes a bf16 value.
 #include "rows_common.h"
 
 namespace ydet {
@@ -22,7 +24,9 @@ struct GradArgs {
     float* part;            // [workgroups][2][C] partial sums of dw and db, or null
     long long rows;
     int C, dy_ld, x_ld, dx_ld, param_dtype;
+    int more;               // the partial sums hold those of the rows before these
 };
+constexpr int kChain = 1024;
 
 template <typename T, bool RAG, int LPR, int CH, int RPT>
 __global__ __launch_bounds__(kThreads) void norm_grad_kernel(const GradArgs a) {
@@ -113,8 +117,10 @@ __global__ __launch_bounds__(kThreads) void norm_grad_kernel(const GradArgs a) {
 #pragma unroll
             for (int i = 0; i < VEC; ++i)
                 if (col + i < a.C) {
-                    part[col + i] = dw[c * VEC + i];
-                    part[a.C + col + i] = db[c * VEC + i];
+                    float& pw = part[col + i];
+                    float& pb = part[a.C + col + i];
+                    pw = a.more ? pw + dw[c * VEC + i] : dw[c * VEC + i];
+                    pb = a.more ? pb + db[c * VEC + i] : db[c * VEC + i];
                 }
         }
     } else {
@@ -132,7 +138,8 @@ __global__ __launch_bounds__(kThreads) void norm_grad_kernel(const GradArgs a) {
                 float s = 0.f;
 #pragma unroll 4
                 for (int k = 0; k < G; ++k) s += meet[k * W + col];
-                part[which * a.C + col] = s;
+                float& to = part[which * a.C + col];
+                to = a.more ? to + s : s;
             }
         }
     }
@@ -181,8 +188,17 @@ static int grad_blocks(long long rows) {
 template <typename T, bool RAG, int LPR, int CH>
 static int launch_grad(const GradArgs& a, int blocks, hipStream_t stream) {
     constexpr int RPT = CH == 1 ? 2 : 1;
-    hipLaunchKernelGGL((norm_grad_kernel<T, RAG, LPR, CH, RPT>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
-    YDET_CHECK_LAUNCH("layer norm gradient");
+    static_assert(kChain % RPT == 0, "rows of a lane group");
+    const long long step = a.part ? (long long)blocks * (kThreads / LPR) * kChain : a.rows;
+    for (long long row = 0; row < a.rows; row += step) {
+        GradArgs b = a;
+        b.rows = a.rows - row < step ? a.rows - row : step;
+        b.dy += row * a.dy_ld * (long long)sizeof(T), b.x += row * a.x_ld * (long long)sizeof(T);
+        if (a.dx) b.dx += row * a.dx_ld * (long long)sizeof(T);
+        b.mean += row, b.rstd += row, b.more = row > 0;
+        hipLaunchKernelGGL((norm_grad_kernel<T, RAG, LPR, CH, RPT>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, b);
+        YDET_CHECK_LAUNCH("layer norm gradient");
+    }
     return YDET_OK;
 }
 
