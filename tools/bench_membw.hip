@@ -1,6 +1,6 @@
 // What a hand-written streaming kernel gets out of HBM on this GPU, on the working sets of the HBM-bound layers
 // (stand-alone tool, not part of libydet.so):
-//   hipcc --offload-arch=gfx950 -O3 tools/bench_membw.hip -o build/bench_membw && build/bench_membw [quick]
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/bench_membw.hip -o build/bench_membw && build/bench_membw [quick]
 //
 // Kernels: 16 bytes per lane, 256-thread workgroups, a persistent grid-stride loop; per wave-instruction 1 KiB contiguous.
 //   copy   c[i] = a[i]                 (1 read, 1 write: a layer that moves its map in and out)

@@ -1,5 +1,5 @@
 // Sustained bf16 MFMA rate of the whole chip with operands in registers (debugging aid, not part of libydet.so):
-//   hipcc --offload-arch=gfx950 -O2 tools/bench_mfma.hip -o tools/bin/bench_mfma && tools/bin/bench_mfma
+//   hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops tools/bench_mfma.hip -o tools/bin/bench_mfma && tools/bin/bench_mfma
 // Every SIMD runs WAVES waves that issue independent MFMAs back to back for about a tenth of a second; printed per
 // instruction shape: TFLOP/s over the wall time of the launch (the last column is the first wave's own span over that
 // time: below the clock when the waves of a SIMD take turns).  What the matrix pipes sustain under power limits is the

@@ -1,5 +1,5 @@
 // Issue cost of single VALU instructions on gfx950 (debugging aid, not part of libydet.so):
-//   hipcc --offload-arch=gfx950 -O2 tools/bench_valu.hip -o tools/bin/bench_valu && tools/bin/bench_valu
+//   hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops tools/bench_valu.hip -o tools/bin/bench_valu && tools/bin/bench_valu
 // One wave per SIMD runs 8 independent chains x 4096 repetitions of one instruction between two s_memtime stamps;
 // printed: shader cycles per wave-instruction.
 #include <hip/hip_runtime.h>

@@ -1,5 +1,5 @@
 // Stand-alone timing trace of conv_dma_kernel (debugging aid, not part of libydet.so):
-//   hipcc --offload-arch=gfx950 -O3 -Iinclude -Iyolo_amd/csrc tools/conv_trace.hip -o build/conv_trace
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -Iinclude -Iyolo_amd/csrc tools/conv_trace.hip -o build/conv_trace
 //   build/conv_trace N H W Cin Cout k stride
 // Prints, for a few workgroups, the cycle stamps relative to the earliest workgroup start.
 #define YDET_TRACE 1
