@@ -936,3 +936,30 @@ def test_parameter_gradients_of_very_many_rows():
     assert float(db) == 255 and float(dw) == 3 * 255
     # dx = r (g - g - xh g xh): with one channel and these statistics, -9 dy at the marks and nothing elsewhere
     assert torch.equal(dx[marks, 0], -9 * dy[marks, 0]) and int((dx != 0).sum()) == 8
+
+
+def test_lost_derivatives_are_errors():
+    """Inputs that require a gradient give the 8-bit operators' results bit for bit, and an error where a gradient is asked for; a
+    forward-mode tangent is an error everywhere."""
+    from torch.autograd import forward_ad
+    g = gen(31)
+    x, res, w = randn(g, 50, 48), randn(g, 50, 20), randn(g, 48)
+    lin = ops.LinearI8.quantize(randn(g, 20, 48))
+    xl, rl, wl = (t.clone().requires_grad_(True) for t in (x, res, w))
+    q, s = ops.layer_norm_quantize(x, w)
+    ql, sl = ops.layer_norm_quantize(xl, wl)
+    assert torch.equal(q, ql) and torch.equal(s, sl) and not s.requires_grad
+    want, y = ops.matmul_i8(q, s, lin, res=res, out_dtype=F32), ops.matmul_i8(ql, sl, lin, res=rl, out_dtype=F32)
+    want2, y2 = ops.linear_i8(x, lin, act="silu"), ops.linear_i8(xl, lin, act="silu")
+    assert torch.equal(want, y) and torch.equal(want2, y2)
+    for out in (sl, y, y2):
+        with pytest.raises(NotImplementedError, match="has no gradient"):
+            out.sum().backward()
+    with torch.no_grad():
+        assert not ops.linear_i8(xl, lin).requires_grad
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, x)
+        for call in (lambda: ops.layer_norm(d), lambda: ops.layer_norm(xl, forward_ad.make_dual(w, w)), lambda: ops.linear_i8(d, lin)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        assert torch.equal(ops.layer_norm(x, w), ops.layer_norm(xl, wl).detach())

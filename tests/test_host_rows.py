@@ -220,3 +220,92 @@ def test_few_rows_in_place_need_a_workspace():
     # other types of rows and output
     assert not meets(dtype=0, out=1, x_ld=128, y_ld=256, y_coff=128) and meets(dtype=0, out=1, x_ld=128, y_ld=256, y_coff=127)
     assert not meets(rows=1, y=P + 128) and meets(rows=1, y=P + 126)
+
+
+# ---- derivatives that the operators do not have are errors, not constants (the library's calls are left out: values do not matter) --
+@pytest.fixture
+def no_launches(monkeypatch):
+    monkeypatch.setattr(ops, "_need_cuda", lambda *t: None)
+    monkeypatch.setattr(ops, "_launch", lambda dev, call, *args: 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+
+
+def _operators():
+    """name -> (call of a floating [4, 32] tensor in every place that takes one, whether it has a gradient)"""
+    lin = ops.LinearI8(torch.ones(8, 32, dtype=torch.int8), torch.ones(8))
+    q, s, x = torch.ones(4, 32, dtype=torch.int8), torch.ones(4), torch.ones(4, 32)
+    F = torch.float32
+    return {"layer_norm": lambda t: ops.layer_norm(t), "layer_norm weight": lambda t: ops.layer_norm(x, t[0]),
+            "layer_norm bias": lambda t: ops.layer_norm(x, None, t[0]), "layer_norm_forward": lambda t: ops.layer_norm_forward(t)[0],
+            "layer_norm_backward dy": lambda t: ops.layer_norm_backward(t, x, s, s)[0],
+            "layer_norm_backward rstd": lambda t: ops.layer_norm_backward(x, x, s, t[:, 0])[0],
+            "quantize_rows": lambda t: ops.quantize_rows(t)[1], "layer_norm_quantize": lambda t: ops.layer_norm_quantize(t)[1],
+            "layer_norm_quantize weight": lambda t: ops.layer_norm_quantize(x, t[0])[1],
+            "matmul_i8 scale": lambda t: ops.matmul_i8(q, t[:, 0], lin, out_dtype=F), "matmul_i8 res": lambda t: ops.matmul_i8(q, s, lin, res=t[:, :8], out_dtype=F),
+            "linear_i8": lambda t: ops.linear_i8(t, lin), "linear_i8 res": lambda t: ops.linear_i8(x, lin, res=t[:, :8])}
+
+
+NAMES = ["layer_norm", "layer_norm weight", "layer_norm bias", "layer_norm_forward", "layer_norm_backward dy", "layer_norm_backward rstd",
+         "quantize_rows", "layer_norm_quantize", "layer_norm_quantize weight", "matmul_i8 scale", "matmul_i8 res", "linear_i8", "linear_i8 res"]
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_forward_mode_is_refused(no_launches, name):
+    from torch.autograd import forward_ad as fwd
+    call = _operators()[name]
+    x = torch.ones(4, 32)
+    with fwd.dual_level():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(fwd.make_dual(x, x))
+        call(x)                                         # (nothing dual: as ever)
+        with torch.no_grad():
+            call(x)
+    call(x)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.jvp(call, (x,), (x,))
+
+
+def test_no_dimension_is_refused(no_launches):
+    for grad in (False, True):
+        with pytest.raises(ValueError, match="at least one channel"):
+            ops.layer_norm(torch.tensor(1.0, requires_grad=grad))
+
+
+def test_forward_mode_through_the_backward_pass_is_refused(no_launches):
+    from torch.autograd import forward_ad as fwd
+    x = torch.ones(4, 32, requires_grad=True)
+    with fwd.dual_level():
+        y = ops.layer_norm(x)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(y, x, fwd.make_dual(torch.ones(4, 32), torch.ones(4, 32)))
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning", "ignore::DeprecationWarning")
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("name", NAMES)
+def test_tracing_is_refused(no_launches, name, grad):
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(_operators()[name], torch.ones(4, 32, requires_grad=grad), check_trace=False)
+
+
+@pytest.mark.parametrize("name", [n for n in NAMES if n.split()[0] in ("quantize_rows", "layer_norm_quantize", "matmul_i8", "linear_i8")])
+def test_gradients_of_8_bit_operators_are_errors(no_launches, name):
+    call = _operators()[name]
+    x = torch.ones(4, 32)
+    assert not call(x).requires_grad
+    leaf = x.clone().requires_grad_(True)
+    with torch.no_grad():
+        assert not call(leaf).requires_grad
+    assert not call(leaf.detach()).requires_grad
+    y = call(leaf)                                      # the call itself is as before
+    with pytest.raises(NotImplementedError, match=f"{'quantize_rows' if 'quantize' in name else name.split()[0]} has no gradient"):
+        (y.sum() + leaf.sum()).backward()
+    assert leaf.grad is None
+
+
+def test_no_gradient_through_a_block_of_8_bit_operators(no_launches):
+    lin = ops.LinearI8(torch.ones(8, 32, dtype=torch.int8), torch.ones(8))
+    w = torch.ones(32, requires_grad=True)
+    y = ops.matmul_i8(*ops.layer_norm_quantize(torch.ones(4, 32), w), lin, out_dtype=torch.float32)
+    with pytest.raises(NotImplementedError, match="has no gradient"):
+        y.sum().backward()

@@ -6,6 +6,7 @@ here synchronises with the host.
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _ffi
 
@@ -283,8 +284,43 @@ def voc_match(boxes, members, group_start, gt_boxes, gt_difficult, gt_start, ovt
 
 # ---- operators over the channels of every pixel ----------------------------------------------------------------------
 # Tensors are [..., C]: any leading dimensions, the channels last (an NHWC map, or a channel slice of one).  Rows at one
-# common distance are read where they lie; other strides, and types other than fp32 / bf16, are copied or refused.
+# common distance are read where they lie; other strides, and types other than fp32 / bf16, are copied or refused.  What they
+# cannot pass on is an error instead of a lost derivative: forward-mode tangents (_no_tangents), tracing (_no_trace), gradients of
+# the 8-bit operators (_without_gradient).
 MAX_ROW = 8192      # channels of a row that layer_norm and quantize_rows take
+
+
+def _no_tangents(what, *ts):
+    """Raises if one of the tensors carries a forward-mode tangent.  (Called where a dual level is open.)"""
+    for t in ts:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
+def _no_trace(what, size):
+    """size: of a dimension, a tensor while torch.jit.trace records, which would keep the result as a constant."""
+    if type(size) is not int:
+        raise RuntimeError(f"{what} cannot be traced")
+
+
+class _NoGradient(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, what, y, *inputs):
+        ctx.what = what
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        raise NotImplementedError(f"{ctx.what} has no gradient: call it under torch.no_grad(), or on detached tensors")
+
+
+def _without_gradient(what, y, *inputs):
+    """y, in whose place in a recorded graph stands an error for the backward pass if an input requires a gradient."""
+    if torch.is_grad_enabled():
+        for t in inputs:
+            if t is not None and t.requires_grad:
+                return _NoGradient.apply(what, y, *inputs)
+    return y
 
 
 def _launch(dev, call, *args):
@@ -302,6 +338,7 @@ def _as_rows(t, what):
     if not shape or not shape[-1]:
         raise ValueError(f"{what} needs at least one channel (shape {tuple(shape)})")
     C = shape[-1]
+    _no_trace(what, C)
     n = shape[0] if len(shape) == 2 else t.numel() // C
     if t.is_contiguous():
         return t, n, C
@@ -364,7 +401,10 @@ def _ln_forward(x, weight, bias, eps, stats):
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
     """Layer normalisation over the last dimension: (y, mean, rstd), y of x's dtype and shape, mean and rstd fp32 of
     x.shape[:-1].  weight, bias: [C] fp32 or bf16, or None.  The variance is an fp32 number: with eps = 0 a row whose variance
-    is below 1.2e-38 counts as constant, and what is divided by its deviation is not finite."""
+    is below 1.2e-38 counts as constant, and what is divided by its deviation is not finite.  No autograd: y is not part of a
+    recorded graph, layer_norm_backward takes the gradients."""
+    if forward_ad._current_level >= 0:
+        _no_tangents("layer_norm_forward", x, weight, bias)
     y, st = _ln_forward(x, weight, bias, eps, True)
     return y, st[0], st[1]
 
@@ -408,6 +448,8 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, need=(True, True, True),
         raise ValueError(f"dy is {dy.dtype} {tuple(dy.shape)}, x is {x.dtype} {tuple(x.shape)}")
     if mean.shape != x.shape[:-1] or rstd.shape != x.shape[:-1] or mean.dtype != torch.float32 or rstd.dtype != torch.float32:
         raise ValueError("mean and rstd are the fp32 tensors that layer_norm_forward returned for x")
+    if forward_ad._current_level >= 0:
+        _no_tangents("layer_norm_backward", dy, x, mean, rstd, weight)
     if not x.device == dy.device == mean.device == rstd.device:
         raise RuntimeError("layer_norm_backward: tensors on different devices")
     mean, rstd = mean.contiguous(), rstd.contiguous()
@@ -424,6 +466,8 @@ class _LayerNorm(torch.autograd.Function):
 
     def _gradients(ctx, dy):
         x, weight, st = ctx.saved_tensors
+        if forward_ad._current_level >= 0:
+            _no_tangents("layer_norm's backward pass", dy, x, weight)
         mean = st.data_ptr()
         return _ln_backward(dy, x, mean, mean + 2 * st.numel(), weight, ctx.needs_input_grad, ctx.bias_dtype) + (None,)
 
@@ -439,19 +483,24 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Layer normalisation over the last dimension, differentiable in x, weight and bias (once).  A recorded graph cannot be
     captured (its leaves' gradients may belong to another stream): a captured training step calls layer_norm_forward and
     layer_norm_backward."""
+    if forward_ad._current_level >= 0:
+        _no_tangents("layer_norm", x, weight, bias)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
         _need_cuda(x)
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("layer_norm: gradients are not recorded during graph capture; call layer_norm_forward and "
                                "layer_norm_backward there")
+        _no_trace("layer_norm", x.numel())          # (inside apply sizes are plain numbers)
         return _LayerNorm.apply(x, weight, bias, eps)
     return _ln_forward(x, weight, bias, eps, False)[0]
 
 
 def _quantize(x, normalize, weight, bias, eps):
     _need_cuda(x)
-    dt = _dt(x)
+    if forward_ad._current_level >= 0:
+        _no_tangents("quantize_rows", x, weight, bias)
+    dt, given = _dt(x), x
     x, n, ld = _as_rows(x, "quantize_rows")
     C, dev, lead = x.shape[-1], x.device, x.shape[:-1]
     w, b, pdt = _params(C, dev, weight, bias)
@@ -462,18 +511,20 @@ def _quantize(x, normalize, weight, bias, eps):
     rc = _launch(dev, _ffi.lib().ydet_quantize_rows_i8, d)
     if rc:
         _ffi.check(rc, "ydet_quantize_rows_i8")
-    return (q if q_ld == C else q[..., :C]), (scale if len(lead) == 1 else scale.view(lead))
+    scale = _without_gradient("quantize_rows", scale if len(lead) == 1 else scale.view(lead), given, weight, bias)
+    return (q if q_ld == C else q[..., :C]), scale
 
 
 def quantize_rows(x):
     """(q, scale): the rows of x [..., C] in 8 bits, q int8 of x's shape (its rows padded with zeros to 16 bytes in memory),
     scale fp32 of x.shape[:-1] with x ~ q * scale.  scale = max|x| / 127; q is the integer nearest x / scale, ties to even.
-    A row with a NaN or an infinity has scale NaN and q = 0."""
+    A row with a NaN or an infinity has scale NaN and q = 0.  For inference: asking for a gradient through it is an error."""
     return _quantize(x, 0, None, None, 0.0)
 
 
 def layer_norm_quantize(x, weight=None, bias=None, eps=1e-5):
-    """quantize_rows(layer_norm(x, weight, bias, eps)) in one pass over x; the normalised values are not rounded in between."""
+    """quantize_rows(layer_norm(x, weight, bias, eps)) in one pass over x; the normalised values are not rounded in between.
+    For inference, like quantize_rows."""
     return _quantize(x, 1, weight, bias, eps)
 
 
@@ -545,8 +596,12 @@ def _product(x, scale, n, ld, lin, act, slope, res, res_mode, out_dtype):
 def matmul_i8(q, scale, lin, act="none", slope=0.1, res=None, res_mode="after", out_dtype=torch.bfloat16):
     """act(q . lin.w^T * scale * lin.scale + lin.bias), [..., N] of out_dtype (bf16 or fp32), from int8 rows q [..., K] and
     their scales [...] (quantize_rows).  act: "none", "leaky" (negative slope `slope`), "silu".  res [..., N] of out_dtype is
-    added after or before the activation (res_mode).  The sums are exact integers.  (For inference: no gradients.)"""
+    added after or before the activation (res_mode).  The sums are exact integers.  For inference: asking for a gradient
+    through it is an error."""
     _need_cuda(q, scale)
+    if forward_ad._current_level >= 0:
+        _no_tangents("matmul_i8", scale, res)
+    given = scale, res
     K, shape = lin.K, q.shape
     if q.dtype != torch.int8 or len(shape) == 0 or shape[-1] != K:
         raise ValueError(f"q is int8 [..., {K}]: got {q.dtype} {tuple(shape)}")
@@ -575,13 +630,16 @@ def matmul_i8(q, scale, lin, act="none", slope=0.1, res=None, res_mode="after", 
     rc = _launch(dev, lib.ydet_matmul_i8, d, _ptr(ws), nbytes)
     if rc:
         _ffi.check(rc, "ydet_matmul_i8")
-    return y if len(lead) == 1 else y.view(lead + (lin.N,))
+    return _without_gradient("matmul_i8", y if len(lead) == 1 else y.view(lead + (lin.N,)), *given)
 
 
 def linear_i8(x, lin, act="none", slope=0.1, res=None, res_mode="after", out_dtype=None):
     """matmul_i8 of a floating map x [..., K], whose rows are quantised (quantize_rows) on the way; out_dtype defaults to x's.
-    The same bits as the two calls; K up to MAX_ROW."""
+    The same bits as the two calls; K up to MAX_ROW.  For inference: asking for a gradient through it is an error."""
     _need_cuda(x)
+    if forward_ad._current_level >= 0:
+        _no_tangents("linear_i8", x, res)
+    given = x, res
     K, shape = lin.K, x.shape
     if shape[-1:] != (K,):
         raise ValueError(f"x is [..., {K}]: got {tuple(shape)}")
@@ -601,4 +659,4 @@ def linear_i8(x, lin, act="none", slope=0.1, res=None, res_mode="after", out_dty
     rc = _launch(dev, lib.ydet_linear_i8, src, d, _ptr(ws), nbytes)
     if rc:
         _ffi.check(rc, "ydet_linear_i8")
-    return y if len(lead) == 1 else y.view(lead + (lin.N,))
+    return _without_gradient("linear_i8", y if len(lead) == 1 else y.view(lead + (lin.N,)), *given)
