@@ -309,3 +309,17 @@ def test_no_gradient_through_a_block_of_8_bit_operators(no_launches):
     y = ops.matmul_i8(*ops.layer_norm_quantize(torch.ones(4, 32), w), lin, out_dtype=torch.float32)
     with pytest.raises(NotImplementedError, match="has no gradient"):
         y.sum().backward()
+
+
+def test_8_bits_are_chosen_where_they_were_measured_to_pay():
+    """Both sides of every border of the rule, with the measured times (us, bf16 kernel / 8 bits)."""
+    from yolo_amd.engine import pointwise_int8_pays as pays
+    better = [(49, 512, 64, 8, 6), (2704, 512, 512, 9.6, 8.7), (1600, 768, 2048, 14, 12), (3249, 1024, 512, 15, 12), (6400, 2048, 512, 26, 24),
+              (6400, 4096, 64, 42, 30), (6656, 1024, 2048, 37, 34), (16384, 1024, 4096, 152, 126), (25600, 512, 1024, 42, 39), (102400, 512, 1024, 161, 135),
+              (46208, 256, 1024, 55, 46), (92416, 384, 1536, 190, 148), (49, 256, 512, 7, 5), (169, 384, 768, 8, 7)]
+    worse = [(5776, 512, 1024, 14, 16), (6400, 512, 64, 9, 10), (6400, 768, 1024, 17, 22), (6400, 1024, 512, 16, 18),
+             (6656, 512, 1024, 15, 18), (16384, 512, 1024, 25, 29), (204800, 512, 1024, 301, 325), (409600, 256, 512, 195, 273), (204800, 256, 1024, 192, 212),
+             (25600, 256, 1024, 29, 30), (102400, 256, 512, 57, 60), (3249, 256, 512, 7, 8), (6656, 256, 1024, 10, 13), (102400, 1024, 256, 81, 115)]
+    assert all(pays(*r[:3]) for r in better)
+    assert not any(pays(*r[:3]) for r in worse)
+    assert all(b > i for *_, b, i in better) and all(b < i for *_, b, i in worse)

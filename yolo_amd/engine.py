@@ -1055,12 +1055,24 @@ def set_pointwise_int8(flag):
 
 
 def pointwise_int8_pays(rows, cin, cout):
-    """Quantisation + product against the bf16 kernels on MI355X, us: the pass that quantises costs the narrow layers of large
-    batches more than the product saves (25600 pixels 512 -> 512: 29 against 24, 102400 pixels 1024 -> 256: 115 against 81).  It
-    pays where few pixels meet a long sum (361 pixels 4096 -> 512: 16 against 42; 400 pixels 512 -> 512: 7.6 against 9.7; 6400
-    pixels 2048 -> 1024: 34 against 37) and where a layer widens (25600 pixels 512 -> 2048: 68 against 88, 102400 pixels 256 ->
-    1024: 97 against 104; but 409600 pixels 128 -> 512: 179 against 166)."""
-    return (rows <= 6400 and cin >= 512) or (cin >= 256 and cout >= 2 * cin)
+    """Whether quantisation + product beat the bf16 kernels on MI355X, by 492 shapes timed both ways (49 to 819200 pixels, 256 to
+    4096 channels; us, 8-bit against bf16).  The pass that quantises costs the narrow layers of large batches more than the product
+    saves (25600 pixels 512 -> 512: 29 against 24, 102400 pixels 1024 -> 256: 115 against 81).  It pays
+      * where few pixels meet a long sum: from 512 input channels up to 2800 pixels (400 pixels 512 -> 512: 7 against 9, 2704 pixels
+        512 -> 1024: 10 and 10; but 5776 pixels 512 -> 1024: 16 against 14), from 1024 up to 4300 (3249 pixels 1024 -> 512: 12 against 15;
+        but 6400 pixels: 18 against 16), from 2048 up to 6400 (361 pixels 4096 -> 512: 15 against 42; 6400 pixels 2048 -> 1024: 33
+        against 36);
+      * where a layer widens at least twofold: from 1024 input channels on (6656 pixels 1024 -> 2048: 34 against 37), from 512 for
+        25600 pixels and more (512 -> 1024: 39 against 42; but 12800 pixels: 26 against 24), fourfold from 256 for 40000 and more
+        (102400 pixels 256 -> 1024: 92 against 103; but 25600 pixels: 30 against 29) -- up to 131072 pixels (204800 pixels 512 -> 1024:
+        325 against 301) -- and, from 256, for up to 400 (169 pixels 256 -> 512: 6 against 7; but 3249 pixels: 8.4 against 7.7)."""
+    if cin >= 512 and rows <= (6400 if cin >= 2048 else 4300 if cin >= 1024 else 2800):
+        return True
+    if cin < 256 or cout < 2 * cin or rows > 131072:
+        return False
+    if cin >= 512:
+        return cin >= 1024 or rows >= 25600
+    return rows <= 400 or (rows >= 40000 and cout >= 4 * cin)
 
 
 def set_head_raw_dtype(mode):
