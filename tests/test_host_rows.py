@@ -309,6 +309,10 @@ def test_no_gradient_through_a_block_of_8_bit_operators(no_launches):
     y = ops.matmul_i8(*ops.layer_norm_quantize(torch.ones(4, 32), w), lin, out_dtype=torch.float32)
     with pytest.raises(NotImplementedError, match="has no gradient"):
         y.sum().backward()
+    # a weight of another type than the bias, which is converted on the way
+    s = ops.layer_norm_quantize(torch.ones(4, 32), torch.ones(32, dtype=torch.bfloat16, requires_grad=True), torch.ones(32))[1]
+    with pytest.raises(NotImplementedError, match="has no gradient"):
+        s.sum().backward()
 
 
 def test_8_bits_are_chosen_where_they_were_measured_to_pay():

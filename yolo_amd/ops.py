@@ -285,7 +285,7 @@ def voc_match(boxes, members, group_start, gt_boxes, gt_difficult, gt_start, ovt
 # ---- operators over the channels of every pixel ----------------------------------------------------------------------
 # Tensors are [..., C]: any leading dimensions, the channels last (an NHWC map, or a channel slice of one).  Rows at one
 # common distance are read where they lie; other strides, and types other than fp32 / bf16, are copied or refused.  What they
-# cannot pass on is an error instead of a lost derivative: forward-mode tangents (_no_tangents), tracing (_no_trace), gradients of
+# cannot pass on is an error instead of a lost derivative: forward-mode tangents (_no_tangents), tracing (_as_rows), gradients of
 # the 8-bit operators (_without_gradient).
 MAX_ROW = 8192      # channels of a row that layer_norm and quantize_rows take
 
@@ -295,12 +295,6 @@ def _no_tangents(what, *ts):
     for t in ts:
         if t is not None and forward_ad.unpack_dual(t).tangent is not None:
             raise NotImplementedError(f"{what} has no forward-mode derivative")
-
-
-def _no_trace(what, size):
-    """size: of a dimension, a tensor while torch.jit.trace records, which would keep the result as a constant."""
-    if type(size) is not int:
-        raise RuntimeError(f"{what} cannot be traced")
 
 
 class _NoGradient(torch.autograd.Function):
@@ -315,12 +309,8 @@ class _NoGradient(torch.autograd.Function):
 
 
 def _without_gradient(what, y, *inputs):
-    """y, in whose place in a recorded graph stands an error for the backward pass if an input requires a gradient."""
-    if torch.is_grad_enabled():
-        for t in inputs:
-            if t is not None and t.requires_grad:
-                return _NoGradient.apply(what, y, *inputs)
-    return y
+    """y, in whose place in a recorded graph stands an error for the backward pass.  (Called where an input requires a gradient.)"""
+    return _NoGradient.apply(what, y, *inputs) if torch.is_grad_enabled() else y
 
 
 def _launch(dev, call, *args):
@@ -338,7 +328,8 @@ def _as_rows(t, what):
     if not shape or not shape[-1]:
         raise ValueError(f"{what} needs at least one channel (shape {tuple(shape)})")
     C = shape[-1]
-    _no_trace(what, C)
+    if type(C) is not int:      # (a tensor while torch.jit.trace records, which would keep the result as a constant)
+        raise RuntimeError(f"{what} cannot be traced")
     n = shape[0] if len(shape) == 2 else t.numel() // C
     if t.is_contiguous():
         return t, n, C
@@ -379,7 +370,8 @@ def _ptr(t):
 
 def _ln_forward(x, weight, bias, eps, stats):
     """(y, statistics): the means of all rows and then their reciprocal deviations in one fp32 buffer, or None."""
-    _need_cuda(x)
+    if not x.is_cuda:
+        _need_cuda(x)
     dt = _dt(x)
     x, n, ld = _as_rows(x, "layer_norm")
     C, dev = x.shape[-1], x.device
@@ -491,16 +483,18 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("layer_norm: gradients are not recorded during graph capture; call layer_norm_forward and "
                                "layer_norm_backward there")
-        _no_trace("layer_norm", x.numel())          # (inside apply sizes are plain numbers)
+        if type(x.numel()) is not int:      # (as in _as_rows; inside apply sizes are plain numbers)
+            raise RuntimeError("layer_norm cannot be traced")
         return _LayerNorm.apply(x, weight, bias, eps)
     return _ln_forward(x, weight, bias, eps, False)[0]
 
 
 def _quantize(x, normalize, weight, bias, eps):
-    _need_cuda(x)
+    if not x.is_cuda:
+        _need_cuda(x)
     if forward_ad._current_level >= 0:
         _no_tangents("quantize_rows", x, weight, bias)
-    dt, given = _dt(x), x
+    dt = _dt(x)
     x, n, ld = _as_rows(x, "quantize_rows")
     C, dev, lead = x.shape[-1], x.device, x.shape[:-1]
     w, b, pdt = _params(C, dev, weight, bias)
@@ -511,7 +505,10 @@ def _quantize(x, normalize, weight, bias, eps):
     rc = _launch(dev, _ffi.lib().ydet_quantize_rows_i8, d)
     if rc:
         _ffi.check(rc, "ydet_quantize_rows_i8")
-    scale = _without_gradient("quantize_rows", scale if len(lead) == 1 else scale.view(lead), given, weight, bias)
+    if len(lead) != 1:
+        scale = scale.view(lead)
+    if x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad):
+        scale = _without_gradient("quantize_rows", scale, x, weight, bias)
     return (q if q_ld == C else q[..., :C]), scale
 
 
@@ -598,10 +595,10 @@ def matmul_i8(q, scale, lin, act="none", slope=0.1, res=None, res_mode="after", 
     their scales [...] (quantize_rows).  act: "none", "leaky" (negative slope `slope`), "silu".  res [..., N] of out_dtype is
     added after or before the activation (res_mode).  The sums are exact integers.  For inference: asking for a gradient
     through it is an error."""
-    _need_cuda(q, scale)
+    if not (q.is_cuda and scale.is_cuda):
+        _need_cuda(q, scale)
     if forward_ad._current_level >= 0:
         _no_tangents("matmul_i8", scale, res)
-    given = scale, res
     K, shape = lin.K, q.shape
     if q.dtype != torch.int8 or len(shape) == 0 or shape[-1] != K:
         raise ValueError(f"q is int8 [..., {K}]: got {q.dtype} {tuple(shape)}")
@@ -630,16 +627,20 @@ def matmul_i8(q, scale, lin, act="none", slope=0.1, res=None, res_mode="after", 
     rc = _launch(dev, lib.ydet_matmul_i8, d, _ptr(ws), nbytes)
     if rc:
         _ffi.check(rc, "ydet_matmul_i8")
-    return _without_gradient("matmul_i8", y if len(lead) == 1 else y.view(lead + (lin.N,)), *given)
+    if len(lead) != 1:
+        y = y.view(lead + (lin.N,))
+    if scale.requires_grad or (res is not None and res.requires_grad):
+        return _without_gradient("matmul_i8", y, scale, res)
+    return y
 
 
 def linear_i8(x, lin, act="none", slope=0.1, res=None, res_mode="after", out_dtype=None):
     """matmul_i8 of a floating map x [..., K], whose rows are quantised (quantize_rows) on the way; out_dtype defaults to x's.
     The same bits as the two calls; K up to MAX_ROW.  For inference: asking for a gradient through it is an error."""
-    _need_cuda(x)
+    if not x.is_cuda:
+        _need_cuda(x)
     if forward_ad._current_level >= 0:
         _no_tangents("linear_i8", x, res)
-    given = x, res
     K, shape = lin.K, x.shape
     if shape[-1:] != (K,):
         raise ValueError(f"x is [..., {K}]: got {tuple(shape)}")
@@ -659,4 +660,8 @@ def linear_i8(x, lin, act="none", slope=0.1, res=None, res_mode="after", out_dty
     rc = _launch(dev, lib.ydet_linear_i8, src, d, _ptr(ws), nbytes)
     if rc:
         _ffi.check(rc, "ydet_linear_i8")
-    return _without_gradient("linear_i8", y if len(lead) == 1 else y.view(lead + (lin.N,)), *given)
+    if len(lead) != 1:
+        y = y.view(lead + (lin.N,))
+    if x.requires_grad or (res is not None and res.requires_grad):
+        return _without_gradient("linear_i8", y, x, res)
+    return y
