@@ -464,7 +464,8 @@ int ydet_preprocess_u8(const ydet_u8_image* images /* device, N entries */, cons
  * rstd = 1 / sqrt(var + eps).  gamma / beta: C values of param_dtype, or NULL (1 / 0).  mean, rstd (rows values each, fp32,
  * both or neither): what the backward pass needs.  y has x's dtype; y may be x.  C <= 8192, rows < 2^31; any ld,
  * and slices at any value's address (a row's result does not depend on where it lies).  eps >= 0; with eps 0 a row whose
- * variance is below 2^-126 counts as constant: its rstd is infinite. */
+ * variance is below 2^-126 counts as constant: its rstd is infinite.  Sums and statistics are fp32 numbers: a row whose sum
+ * passes 3.4e38 becomes NaN, one whose sum of squared differences to the mean does has rstd 0. */
 typedef struct {
     const void* x;
     void* y;

@@ -963,3 +963,14 @@ def test_lost_derivatives_are_errors():
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
         assert torch.equal(ops.layer_norm(x, w), ops.layer_norm(xl, wl).detach())
+
+
+def test_rows_at_the_end_of_single_precision():
+    """Rows whose sums pass the largest number, as documented; the largest rows that do not."""
+    x = torch.tensor([[1e38, 1e38, 1e38, 1e38], [1e19, -1e19, 1e19, 3e19], [1e19, -1e19, 8e18, 2e18], [8e37, 8e37, 8e37, 8e37]], device=DEV)
+    y, mean, rstd = ops.layer_norm_forward(x, None, torch.full((4,), 0.5, device=DEV))
+    assert y[0].isnan().all() and mean[0].isnan()
+    assert float(rstd[1]) == 0 and (y[1] == 0.5).all()
+    y64, xh, r64 = norm64(x[2:3], None, None, 1e-5)
+    within(y[2:3] - 0.5, y64, xh_error(x[2:3], xh, r64) + 4 * U)
+    assert (y[3] == 0.5).all()

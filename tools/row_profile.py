@@ -30,7 +30,7 @@ def cases():
     m.own = True
     more = [dict(op="quant", rows=23104, c=2048, x="bf16", name="quantisation 23104 x 2048"),
             dict(op="ln_quant", rows=23104, c=2048, x="bf16", name="norm + quantisation 23104 x 2048"),
-            dict(op="random", rows=102400, k=256, n=1024, name="product 256 -> 1024, uniform random bytes")]
+            dict(op="memory", rows=102400, k=256, n=1024, name="product, rows from memory")]
     return m, m.listed() + more
 
 
@@ -48,7 +48,7 @@ def run(i):
         states = [torch.randn(c["rows"], c["c"], device="cuda").bfloat16() for _ in range(3)]
         w, b = torch.randn(2, c["c"], device="cuda")
         call = ops.quantize_rows if c["op"] == "quant" else lambda x: ops.layer_norm_quantize(x, w, b)
-    elif c["op"] == "random":
+    elif c["op"] == "memory":
         byte = lambda *s: torch.randint(-128, 128, s, device="cuda", dtype=torch.int8)
         lin = ops.LinearI8(byte(c["n"], c["k"]), torch.rand(c["n"], device="cuda") * 0.01, torch.randn(c["n"], device="cuda"))
         s = torch.rand(c["rows"], device="cuda") * 0.01

@@ -139,10 +139,12 @@ __device__ __forceinline__ void load_channels(const float* ws, const float* bias
 // c ^ ((r >> 1) & 7), so that the 16 rows a fragment read touches fall into 16 different places of the banks.  Stages are filled by
 // LDS-DMA (eight rows an instruction), from rows at any 4-byte address and pitch; rows behind the last pixel and channels behind
 // n_pad lie outside the buffer descriptors, which are checked word by word, and read as zeros.  NST stages; the fragments of a half stage are read while the previous half's MFMAs run.
-// What bounds it: for long K the operands' way through L2 (52 us for 23104 x 4096 -> 512 with 256 x 192 tiles: 1.85 POP/s, where a
-// library product of 8192^3 reaches 2.06), for short K the rows and the output (52 us for 409600 x 128 -> 128 with SiLU and
-// residual: 5.0 TB/s), for many channels and short K the epilogue, about ten operations a value, two of them transcendental
-// (70 us for 102400 x 256 -> 1024, half of which the vector units are busy).
+// What bounds it: for long K the operands' way through L2 (52 us for 23104 x 4096 -> 512 with 256 x 192 tiles: 1.85 POP/s, the matrix
+// units busy 37 % of the time; a library product of 8192^3 reaches 2.26 in bursts of eight and 2.5 in a long train), for short K
+// the rows and the output (51 us for 409600 x 128 -> 128 with SiLU and residual: 5.1 TB/s), for many channels and short K the
+// epilogue, about ten operations a value, two of them transcendental (73 us for 102400 x 256 -> 1024, the vector units busy 63 % of
+// the time, where the rows have just been written and lie in the last-level cache; 93 where they come from memory, whose latency a
+// tile of two stages does not hide; what the bytes are changes neither by more than the clock does).
 template <typename OUT, int BN, int BM, int WAVES_N, int WAVES_M, int NST = 2>
 __global__ __launch_bounds__(64 * WAVES_N * WAVES_M, 2) void tile_kernel(const Args a) {
     constexpr int NW = WAVES_N * WAVES_M, WN = BN / WAVES_N, WM = BM / WAVES_M, FN = WN / 16, FM = WM / 16;
@@ -544,19 +546,19 @@ __global__ __launch_bounds__(256) void align_rows_kernel(const char* x, long lon
     }
 }
 
-// Which kernel takes a product, by rows, channels and K alone; every one gives the same bits.  Measured on 256 CUs, us:
-//   16 x 16 outputs a workgroup, straight from memory, up to two workgroups a CU (1 x 1024 -> 1024: 2.9; 40 x 4096 -> 512: 5.7, in
-//     64 x 128 tiles 12.2; 100 x 1024 -> 512: 3.3 against 5.3);
-//   32 x 32, straight from memory, up to one a CU (400 x 1024 -> 512: 4.6 against 5.4; 200 x 2048 -> 1024: 6.4 against 7.7, but
-//     1600 x 512 -> 512: 6.7 against 4.5);
-//   256 x 192 tiles for K >= 2048 where they leave no quarter of the CUs idle (23104 x 4096 -> 512: 52, in 128 x 128 tiles 73; but
-//     25600 x 1024 -> 512: 32 against 25);
-//   128 x 128 for K >= 1024 with at least a tile a CU (6400 x 1024 -> 1024: 13.3, in 64 x 128 tiles 16.4; with four waves instead of
-//     eight 13.6);
-//   64 x 128 otherwise (409600 x 64 -> 64: 18, in 128 x 128 tiles 28; 409600 x 128 -> 128 with residual: 52 against 62), with a
-//     third stage where there are fewer than two workgroups a CU (2888 x 4096 -> 512: 14.6, with two stages 19.2).
+// Which kernel takes a product, by rows, channels and K alone; every one gives the same bits.  Measured on 256 CUs, us, the kernel
+// alone with three inputs in turn:
+//   16 x 16 outputs a workgroup, straight from memory, up to two workgroups a CU (1 x 1024 -> 1024: 3.2, in 64 x 128 tiles 5.5; 40 x
+//     4096 -> 512: 6.3 against 12.8; 100 x 1024 -> 512: 3.8 against 5.9);
+//   32 x 32, straight from memory, up to one a CU (400 x 1024 -> 512: 5.2, in 64 x 128 tiles 6.2; 200 x 2048 -> 1024: 7.0 against 8.3,
+//     but 1600 x 512 -> 512: 7.3 against 5.1);
+//   256 x 192 tiles for K >= 2048 where they leave no quarter of the CUs idle (23104 x 4096 -> 512: 55, in 128 x 128 tiles 80; but
+//     25600 x 1024 -> 512: 31 against 26);
+//   128 x 128 for K >= 1024 with at least a tile a CU (6400 x 1024 -> 1024: 13.5, in 64 x 128 tiles 16.2);
+//   64 x 128 otherwise (409600 x 64 -> 64: 16, in 128 x 128 tiles 25; 409600 x 128 -> 128 with residual: 49 against 53), with a
+//     third stage where there are fewer than two workgroups a CU (2888 x 4096 -> 512: 14.7, with two stages 18.7).
 // The tile kernels want rows at 4-byte addresses and pitches: others are first copied into the workspace (2888 x 1000 -> 255: 3.4 us
-// and a launch more on top of 6.8).
+// and a launch more on top of 6.7).
 static long long tiles(const Args& a, int bn, int bm) { return (long long)((a.N + bn - 1) / bn) * ((a.M + bm - 1) / bm); }
 static int direct_size(const Args& a) {
     const int cus = current_device_info().cus;

@@ -180,9 +180,11 @@ __global__ __launch_bounds__(kThreads) void row_norm_kernel(const RowArgs a) {
 }
 
 // Workgroups: each walks over rows, weight and bias in its registers.  No more than stay resident where a workgroup reads weight and
-// bias (23104 x 2048 norm + quantisation in bf16, 64 lanes a row: 54 us with four a CU, 72 with one for every four rows; up to 16
-// values a lane leave room for eight a CU), twice as many where it reads none (25600 x 512 quantisation: 10.9 us, with eight 11.6) or
-// takes four rows at a time (409600 x 128 norm: 39.2 us, with eight 41.7).
+// bias: four a CU for rows of more than 4096 values, 32 a lane (5776 x 8192 norm + quantisation in fp32 66 us, with eight 73, with 16
+// 85; 23104 x 4224 in bf16 178 against 181, norm alone 77 against 79; 8192 in bf16 level), eight for shorter ones (23104 x 2048 norm
+// + quantisation in bf16 39 us, with four 49; 51200 x 512 in fp32 level).  Twice as many where it reads none (25600 x 512
+// quantisation 10.3 us, with eight 10.9; 23104 x 4224 103 against 106) or takes four rows at a time (409600 x 128 norm 38.6 us, with
+// eight 41.2).
 template <int MODE, typename T, bool RAG, int LPR, int CH, int RPT>
 static int launch_rows(const RowArgs& a, hipStream_t stream) {
     constexpr int per = kThreads / LPR * RPT, per_cu = !(MODE & kNorm) || RPT > 1 ? 16 : CH * 16 / (int)sizeof(T) > 16 ? 4 : 8;

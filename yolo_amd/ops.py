@@ -393,8 +393,9 @@ def _ln_forward(x, weight, bias, eps, stats):
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
     """Layer normalisation over the last dimension: (y, mean, rstd), y of x's dtype and shape, mean and rstd fp32 of
     x.shape[:-1].  weight, bias: [C] fp32 or bf16, or None.  The variance is an fp32 number: with eps = 0 a row whose variance
-    is below 1.2e-38 counts as constant, and what is divided by its deviation is not finite.  No autograd: y is not part of a
-    recorded graph, layer_norm_backward takes the gradients."""
+    is below 1.2e-38 counts as constant, and what is divided by its deviation is not finite; a row whose sum passes 3.4e38
+    becomes NaN, one whose sum of squared differences does has rstd 0.  No autograd: y is not part of a recorded graph,
+    layer_norm_backward takes the gradients."""
     if forward_ad._current_level >= 0:
         _no_tangents("layer_norm_forward", x, weight, bias)
     y, st = _ln_forward(x, weight, bias, eps, True)
