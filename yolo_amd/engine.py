@@ -1057,7 +1057,7 @@ def set_pointwise_int8(flag):
 def pointwise_int8_pays(rows, cin, cout):
     """Whether quantisation + product beat the bf16 kernels on MI355X, by 492 shapes timed both ways (49 to 819200 pixels, 256 to
     4096 channels; us, 8-bit against bf16).  The pass that quantises costs the narrow layers of large batches more than the product
-    saves (25600 pixels 512 -> 512: 29 against 24, 102400 pixels 1024 -> 256: 115 against 81).  It pays
+    saves (25600 pixels 512 -> 512: 28 against 24, 102400 pixels 1024 -> 256: 105 against 77).  It pays
       * where few pixels meet a long sum: from 512 input channels up to 2800 pixels (400 pixels 512 -> 512: 7 against 9, 2704 pixels
         512 -> 1024: 10 and 10; but 5776 pixels 512 -> 1024: 16 against 14), from 1024 up to 4300 (3249 pixels 1024 -> 512: 12 against 15;
         but 6400 pixels: 18 against 16), from 2048 up to 6400 (361 pixels 4096 -> 512: 15 against 42; 6400 pixels 2048 -> 1024: 33
