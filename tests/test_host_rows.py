@@ -303,6 +303,20 @@ def test_gradients_of_8_bit_operators_are_errors(no_launches, name):
     assert leaf.grad is None
 
 
+@pytest.mark.parametrize("shape", [(4,), (2, 2)])
+def test_results_of_8_bit_operators_may_be_changed_in_place(no_launches, shape):
+    """As before there was an error to record, also where the result is laid out in more than two dimensions."""
+    lin = ops.LinearI8(torch.ones(8, 32, dtype=torch.int8), torch.ones(8))
+    x = torch.ones(*shape, 32, requires_grad=True)
+    for y in (ops.linear_i8(x, lin), ops.quantize_rows(x)[1], ops.matmul_i8(torch.ones(*shape, 32, dtype=torch.int8), *ops.quantize_rows(x)[1:], lin)):
+        y.zero_()
+        y += 1
+        y[..., :1].mul_(2)
+        assert y.shape[:len(shape)] == shape and float(y.detach().flatten()[0]) == 2
+        with pytest.raises(NotImplementedError, match="has no gradient"):
+            y.sum().backward()
+
+
 def test_no_gradient_through_a_block_of_8_bit_operators(no_launches):
     lin = ops.LinearI8(torch.ones(8, 32, dtype=torch.int8), torch.ones(8))
     w = torch.ones(32, requires_grad=True)

@@ -1,11 +1,11 @@
 #!/bin/bash
-# Kernel times and counters of the operators over channels (run through gpurun from the repository root): tools/profile_rows.sh
-# Leaves gpurun_out/prof_rows/{t<case>,c<case><pass>}; afterwards
-#   python3 tools/row_profile.py trace gpurun_out/prof_rows > profiles/row_operators_kernel_times.csv
-#   python3 tools/row_profile.py counters gpurun_out/prof_rows > profiles/row_operators_counters.json
+# Kernel times and counters of the operators over channels, from the repository root: tools/profile_rows.sh <dir>
+# Leaves <dir>/{t<case>,c<case><pass>}; afterwards
+#   python3 tools/row_profile.py trace <dir> > profiles/row_operators_kernel_times.csv
+#   python3 tools/row_profile.py counters <dir> > profiles/row_operators_counters.json
 # Counters never share a run with a trace, nor more than one block's worth a pass.
 set -e
-out=gpurun_out/prof_rows
+out=$1
 mkdir -p $out
 export TMPDIR=/tmp
 n=$(python3 tools/row_profile.py count)

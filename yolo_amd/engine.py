@@ -1065,7 +1065,7 @@ def pointwise_int8_pays(rows, cin, cout):
       * where a layer widens at least twofold: from 1024 input channels on (6656 pixels 1024 -> 2048: 34 against 37), from 512 for
         25600 pixels and more (512 -> 1024: 39 against 42; but 12800 pixels: 26 against 24), fourfold from 256 for 40000 and more
         (102400 pixels 256 -> 1024: 92 against 103; but 25600 pixels: 30 against 29) -- up to 131072 pixels (204800 pixels 512 -> 1024:
-        325 against 301) -- and, from 256, for up to 400 (169 pixels 256 -> 512: 6 against 7; but 3249 pixels: 8.4 against 7.7)."""
+        325 against 301) -- and, from 256, for up to 400 (169 pixels 256 -> 512: 6 against 7; but 3249 pixels: 8.0 against 7.3)."""
     if cin >= 512 and rows <= (6400 if cin >= 2048 else 4300 if cin >= 1024 else 2800):
         return True
     if cin < 256 or cout < 2 * cin or rows > 131072:

@@ -299,9 +299,9 @@ def _no_tangents(what, *ts):
 
 class _NoGradient(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, what, y, *inputs):
+    def forward(ctx, what, held, *inputs):
         ctx.what = what
-        return y
+        return held[0].detach()     # (an output of its own: as a tensor argument it would be a view that may not be changed in place)
 
     @staticmethod
     def backward(ctx, dy):
@@ -310,7 +310,7 @@ class _NoGradient(torch.autograd.Function):
 
 def _without_gradient(what, y, *inputs):
     """y, in whose place in a recorded graph stands an error for the backward pass.  (Called where an input requires a gradient.)"""
-    return _NoGradient.apply(what, y, *inputs) if torch.is_grad_enabled() else y
+    return _NoGradient.apply(what, (y,), *inputs) if torch.is_grad_enabled() else y
 
 
 def _launch(dev, call, *args):
